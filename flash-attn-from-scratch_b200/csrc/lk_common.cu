@@ -13,6 +13,7 @@
 namespace lk {
 
 __device__ int g_status[4];
+__device__ int g_bad_index[4];
 __device__ unsigned long long g_wait_limit_ns = 1000000000ull;
 
 namespace {
@@ -58,6 +59,11 @@ int bind_device(int dev) {
 
 int bind_stream(cudaStream_t stream) {
   if (stream == nullptr) return t_bound_device >= 0 ? LK_OK : bind_device(0);
+  // A capturing stream may not be asked for its device (the query ends the capture with an
+  // error): the device that lk_set_device or an earlier call bound is taken.
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone && t_bound_device >= 0)
+    return LK_OK;
   int dev = -1;
   const int st = cuda_status(cudaStreamGetDevice(stream, &dev));
   if (st != LK_OK) return st;
@@ -209,6 +215,10 @@ int lk_device_status(int* out4) {
   if (st != LK_OK) return st;
   st = lk::cuda_status(cudaMemcpyFromSymbol(h, lk::g_status, sizeof(h)));
   if (st != LK_OK) return st;
+  if (h[0] == 0) {
+    st = lk::cuda_status(cudaMemcpyFromSymbol(h, lk::g_bad_index, sizeof(h)));
+    if (st != LK_OK) return st;
+  }
   if (out4)
     for (int i = 0; i < 4; ++i) out4[i] = h[i];
   return h[0];
@@ -235,6 +245,8 @@ int lk_clear_device_status(void) {
   if (st != LK_OK) return st;
   // A split GEMM launch that gave up may have left its tail counters non-zero.
   st = lk::cuda_status((cudaError_t)lk::gemm::reset_split_workspaces());
+  if (st != LK_OK) return st;
+  st = lk::cuda_status(cudaMemcpyToSymbol(lk::g_bad_index, z, sizeof(z)));
   if (st != LK_OK) return st;
   return lk::cuda_status(cudaMemcpyToSymbol(lk::g_status, z, sizeof(z)));
 }

@@ -28,8 +28,15 @@ namespace lk {
 // ---------------------------------------------------------------------------------------------
 extern __device__ int g_status[4];
 
+// A second word of the same layout for an index out of range in the caller's device data (a
+// cache slot, a page id, a position, a length): the kernel skips or clamps the access and
+// records the first one here.  Kept apart from g_status, which makes the waits of every other
+// kernel give up.
+extern __device__ int g_bad_index[4];
+
 enum DeviceCode : int {
   kDevOk = 0,
+  kDevBadIndex = 1,  // matches LK_ERR_INVALID_ARG in the public header
   kDevTimeout = 4,  // matches LK_ERR_TIMEOUT in the public header
 };
 
@@ -59,6 +66,14 @@ __device__ __forceinline__ void record_failure(int code, int site) {
     g_status[3] = (int)threadIdx.x;
   }
   __threadfence();
+}
+
+static __device__ __noinline__ void record_bad_index(int site) {
+  if (atomicCAS(&g_bad_index[0], 0, kDevBadIndex) == 0) {
+    g_bad_index[1] = site;
+    g_bad_index[2] = (int)blockIdx.x;
+    g_bad_index[3] = (int)threadIdx.x;
+  }
 }
 
 __device__ __forceinline__ bool device_failed() {

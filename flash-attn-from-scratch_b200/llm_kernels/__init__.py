@@ -10,6 +10,9 @@ kernels reached through the C ABI in ``include/llm_kernels_b200.h``.
 >>> out = llm_kernels.int8_gemm_dequant_fwd(A_q, B_q, sa, sb)
 >>> out = llm_kernels.fused_rmsnorm_linear(x, w_norm, w_lin)
 >>> out = llm_kernels.flash_attn_with_grad(q, k, v, causal=True); out.sum().backward()
+>>> q, k = llm_kernels.rotary_embed(q, k, positions, table)
+>>> q = llm_kernels.paged_kv_append(k, v, k_cache, v_cache, slots, q=q, positions=positions, cos_sin=table)
+>>> out = llm_kernels.paged_attention(q, k_cache, v_cache, block_table, lengths)
 
 There is no CPU or PyTorch fallback: every op runs its CUDA kernel or raises.
 """
@@ -30,6 +33,8 @@ from .int8_gemm import (
     int8_gemm_i32,
     quantize_symmetric,
 )
+from .paged import cache_slots, paged_attention, paged_kv_append, shared_prefix_attention
+from .rotary import rotary_embed, rotary_table
 
 
 class FlashAttention(nn.Module):
@@ -131,4 +136,12 @@ __all__ = [
     "FlashAttnFunction",
     "flash_attn_with_grad",
     "flash_attn_forward_lse",
+    # positions (training and serving)
+    "rotary_embed",
+    "rotary_table",
+    # serving from a paged key/value cache
+    "cache_slots",
+    "paged_kv_append",
+    "paged_attention",
+    "shared_prefix_attention",
 ]

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,7 +25,7 @@ LK_ERR_ALIGNMENT = 5
 LK_ERR_SCRATCH_LIMIT = 6
 LK_PEER_HANDLE_BYTES = 64  # include/llm_kernels_b200.h
 
-LK_F32, LK_F16, LK_BF16, LK_I8, LK_I32 = 0, 1, 2, 3, 4
+LK_F32, LK_F16, LK_BF16, LK_I8, LK_I32, LK_I64 = 0, 1, 2, 3, 4, 5
 
 # Failure-path test hooks (lk_inject).
 LK_INJECT_NONE, LK_INJECT_FA_DROP_LOAD, LK_INJECT_GEMM_DROP_LOAD, LK_INJECT_SPLIT_SKIP_PUBLISH = 0, 1, 2, 3
@@ -35,6 +36,7 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
 _pi64 = ctypes.POINTER(ctypes.c_int64)
+_b64 = ctypes.c_char_p  # const int64_t* given as packed bytes (pack_i64): no array object per call
 
 # name -> (restype, argtypes); mirrors include/llm_kernels_b200.h one for one.
 SIGNATURES = {
@@ -77,6 +79,25 @@ SIGNATURES = {
     "lk_flash_attn_bwd": (
         _i,
         [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _i, _f, _p],
+    ),
+    "lk_rotary_embed": (
+        _i,
+        [_p, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _b64, _p, _i64, _i64, _i64, _b64, _i, _i, _p],
+    ),
+    "lk_paged_kv_append": (
+        _i,
+        [_p, _p, _p, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _b64, _p, _i64, _i64,
+         _i64, _b64, _i, _p],
+    ),
+    "lk_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "lk_paged_attention": (
+        _i,
+        [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p, _i64, _p],
+    ),
+    "lk_shared_prefix_attention": (
+        _i,
+        [_p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p,
+         _i64, _p],
     ),
     "lk_rmsnorm_linear_fold": (_i, [_p, _i, _p, _p, _i, _i64, _i64, _p]),
     "lk_rmsnorm_linear": (_i, [_p, _i64, _p, _p, _i64, _i, _i64, _i64, _i64, _f, _p, _p]),
@@ -143,6 +164,11 @@ def i64_array(vals) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
 
 
+def pack_i64(*vals) -> bytes:
+    """int64 values as the bytes that a ``const int64_t*`` parameter points to."""
+    return struct.pack("%dq" % len(vals), *vals)
+
+
 _tls = threading.local()
 
 
@@ -154,10 +180,12 @@ def set_device(index: int) -> None:
 
 
 def device_status() -> tuple[int, int, int, int]:
-    """Synchronises and returns the device status word (code, site, block, thread)."""
+    """Synchronises and returns the device status word (code, site, block, thread): code 4 for a
+    pipeline wait that ran out, 1 for an index out of range in device data (a cache slot, a page
+    id, a position, a length)."""
     out = (ctypes.c_int * 4)()
     st = load().lk_device_status(out)
-    if st not in (LK_OK, LK_ERR_TIMEOUT):
+    if st not in (LK_OK, LK_ERR_TIMEOUT, LK_ERR_INVALID_ARG):
         raise LKError("lk_device_status", st)
     return tuple(out)
 

@@ -46,7 +46,7 @@ typedef enum {
 } lk_status;
 
 /* ---- dtype codes ------------------------------------------------------------------------- */
-typedef enum { LK_F32 = 0, LK_F16 = 1, LK_BF16 = 2, LK_I8 = 3, LK_I32 = 4 } lk_dtype;
+typedef enum { LK_F32 = 0, LK_F16 = 1, LK_BF16 = 2, LK_I8 = 3, LK_I32 = 4, LK_I64 = 5 } lk_dtype;
 
 /* Human-readable name of a status code (static string). */
 LK_API const char* lk_status_string(int status);
@@ -65,6 +65,9 @@ LK_API int lk_set_device(int device);
 /* Synchronises the current device, then copies its status word into out4 (may be NULL):
  * out4[0] = lk_status of the first device failure (0 = none), out4[1] = failure site id,
  * out4[2] = blockIdx.x, out4[3] = threadIdx.x of the thread that recorded it.
+ * LK_ERR_INVALID_ARG means that a kernel met an index out of range in the caller's device data
+ * (sites 301 position, 302 cache slot, 311 page id, 312 sequence length); it made no access
+ * there, and other kernels are not affected.
  * Returns out4[0] (or LK_ERR_CUDA). */
 LK_API int lk_device_status(int* out4);
 
@@ -316,6 +319,82 @@ LK_API int lk_fused_rmsnorm_linear(const void* X, const void* W_norm, const void
 LK_API int lk_rmsnorm_linear_noalloc(const void* x, int64_t x_ld, const void* w_fold, void* y,
                                      int64_t y_ld, int dtype, int64_t rows, int64_t d_in,
                                      int64_t d_out, float eps, void* stream);
+
+/* ---- rotary position embedding ------------------------------------------------------------ *
+ * No counterpart in the reference, whose models have no positions.
+ * Rotates the first 2 * pairs values of every head of q [B, S, H, D] and k [B, S, H_kv, D] into
+ * q_out and k_out (which may be q and k themselves); the others are copied.  Pair i is
+ * (x[i], x[i + pairs]), or (x[2i], x[2i + 1]) when interleaved; with p the token's position on
+ * the pair's axis and (c, s) = cos_sin[p][i] (fp32 [table_rows][pairs][2], 8-byte aligned):
+ *     a' = a c - b s,   b' = b c + a s          (fp32, rounded once; inverse: -s, the gradient)
+ *   strides:   12 element strides, (b, s, h) of q, q_out, k, k_out; the d strides are 1.  Rows
+ *              on 16 bytes with D % 16 == 0 and pairs % 8 == 0 take 16-byte accesses.
+ *   positions: LK_I32 or LK_I64, element strides pos_strides = (axis, b, s), axes of 1 to 4; with
+ *              more than one, sections[a] of the pairs (in order, their sum is pairs) belong to
+ *              axis a.  A position outside [0, table_rows) is clamped and reported
+ *              (lk_device_status).
+ * H or H_kv may be 0 (that tensor's pointers and strides are then not used; strides still holds
+ * 12 values).  dtype LK_F16 or LK_BF16. */
+LK_API int lk_rotary_embed(const void* q, void* q_out, const void* k, void* k_out, const int64_t* strides, int dtype,
+                           int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, const void* positions,
+                           int pos_dtype, const int64_t* pos_strides, const float* cos_sin, int64_t table_rows,
+                           int64_t pairs, int64_t axes, const int64_t* sections, int interleaved, int inverse,
+                           void* stream);
+
+/* ---- append to a paged key/value cache ---------------------------------------------------- *
+ * No counterpart in the reference, which keeps no cache.
+ * For each of T tokens with 0 <= slots[t] < num_pages * page_size writes k[t] (rotated as by
+ * lk_rotary_embed) and v[t] into row slots[t] % page_size of page slots[t] / page_size; a
+ * negative slot is padding and writes nothing, one past the cache writes nothing and is
+ * reported.  q [T, H, D] (H may be 0) is rotated into q_out for every token.  No two tokens may
+ * name the same slot.
+ *   strides:  14 element strides: (t, h) of q, q_out, k, v, then (page, row, h) of k_cache and
+ *             v_cache; the d strides are 1.
+ *   slots:    LK_I32 or LK_I64, contiguous.
+ *   cos_sin:  NULL appends k as it is (H must be 0); otherwise the arguments of lk_rotary_embed
+ *             with pos_strides = (axis, unused, t). */
+LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const void* v, void* k_cache, void* v_cache,
+                              const int64_t* strides, int dtype, int64_t T, int64_t H, int64_t H_kv, int64_t D,
+                              int64_t num_pages, int64_t page_size, const void* slots, int slots_dtype,
+                              const void* positions, int pos_dtype, const int64_t* pos_strides, const float* cos_sin,
+                              int64_t table_rows, int64_t pairs, int64_t axes, const int64_t* sections,
+                              int interleaved, void* stream);
+
+/* ---- attention over a paged key/value cache ----------------------------------------------- *
+ * No counterpart in the reference, whose attention reads contiguous keys
+ * (kernels/flash_attn/flash_attn_fwd.py:131-156).
+ * q [B, n, H, D] holds each sequence's n newest tokens, already in its pages.  Sequence b has
+ * lengths[b] keys; key j lies in row j % page_size of page block_table[b * table_ld +
+ * j / page_size].  Token i sees the keys j < lengths[b] - n + i + 1; query head h reads K/V head
+ * h / (H / H_kv):
+ *     out = softmax(scale q K^T) V,   lse[b][i][h] = ln sum_j exp(scale q.k_j)   (lse may be NULL)
+ * A token that sees no key gives 0 and -inf.  Table entries past a sequence's last page are not
+ * read; what lies behind its last key in a page never reaches the result.  A page id outside
+ * [0, num_pages) counts as zeros and a length past table_cols * page_size is cut to that; both
+ * are reported (lk_device_status).
+ *   strides:   12 element strides: (b, n, h) of q and out, (page, row, h) of k_cache and v_cache,
+ *              multiples of 8 with 16-byte aligned bases; the d strides are 1.
+ *   D:         a multiple of 8 up to 128.  dtype LK_F16 or LK_BF16.  softmax_scale <= 0 = D^-0.5.
+ *   workspace: lk_paged_attention_workspace_bytes(...) bytes, 256-byte aligned, zeroed once
+ *              before its first use; every call leaves its counters at zero again, so calls on
+ *              one stream share it and calls that can overlap do not.
+ *
+ * lk_shared_prefix_attention: the same for a batch whose sequences share their first
+ * prefix_length keys, held in the pages prefix_pages[0 ..]; every token sees all of them, and
+ * they are read and multiplied once for the whole batch.  block_table and lengths name what
+ * follows the prefix, from the start of a page of its own; lengths[b] may be 0. */
+LK_API int64_t lk_paged_attention_workspace_bytes(int64_t H, int64_t H_kv, int64_t D);
+LK_API int lk_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                              int64_t table_ld, int64_t table_cols, const int32_t* lengths, void* out, float* lse,
+                              const int64_t* strides, int dtype, int64_t B, int64_t n, int64_t H, int64_t H_kv,
+                              int64_t D, int64_t num_pages, int64_t page_size, float softmax_scale, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+LK_API int lk_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache,
+                                      const int32_t* prefix_pages, int64_t prefix_length, const int32_t* block_table,
+                                      int64_t table_ld, int64_t table_cols, const int32_t* lengths, void* out,
+                                      float* lse, const int64_t* strides, int dtype, int64_t B, int64_t n, int64_t H,
+                                      int64_t H_kv, int64_t D, int64_t num_pages, int64_t page_size,
+                                      float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
