@@ -1,106 +1,466 @@
-// paged_attn.cu — attention of each sequence's newest tokens to its pages of a key/value cache.
+// paged_attn.cu — attention of each sequence's newest tokens to its pages of a key/value cache:
+// the kernel for up to 16 query rows per K/V head (single tokens, drafted tokens).
 //
 // Query i of the n newest tokens of a sequence of L keys sees its keys below L - n + i + 1 (and,
 // with a shared prefix, all of the prefix):  o = sum_j p_j v_j / sum_j p_j with
 // p_j = exp(scale q.k_j - m), lse = m + ln sum_j p_j; a row that sees nothing gives 0 and -inf.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+//
+// Bound: memory.  Each key and value is read once for at most 16 rows (4 D bytes for 64 D flops
+// per key and head at 16 rows: 16 flop/byte, and the card's balance is ~250), so the work is to
+// keep reads in flight.  Four warps of a block take 16 keys each of every 64-key unit and run
+// without any barrier between them until an item ends: a warp has its own ring of stages in
+// shared memory, filled by 16-byte cp.async -- row by row through the block table, so pages of
+// any size and caches of any stride take the same path, and rows behind the last key are filled
+// with zeros instead of read -- and its own running (m, l, O), kept in registers.  The rows of
+// a K/V head's query group fill the 16 rows of mma.sync's A operand, and S's accumulator layout
+// is P's operand layout, so P never leaves registers.  (tcgen05 would need 128 rows and a trip
+// through tensor memory for the same 16; its throughput is not what bounds this kernel.)
+// Loads run ahead across the ends of items, so short sequences do not drain the ring.
+#include <atomic>
 
 #include "lk_abi.h"
-#include "lk_sm100.cuh"
+#include "paged_common.cuh"
 
 namespace lk {
 namespace paged {
 
-enum Site : int {
-  kSitePage = 311,    // a page id outside the cache
-  kSiteLength = 312,  // a length past the block table's room
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;              // query rows of an item
+constexpr int kGroup = 16;             // keys of one warp's step
+constexpr int kUnit = kWarps * kGroup;  // keys of a unit
+constexpr int kStages = 3;
+constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
+
+template <int DP>
+struct Cfg {
+  static constexpr int kTile = kGroup * DP * 2;              // bytes of a warp's K or V tile
+  static constexpr int kRing = kWarps * kStages * 2 * kTile;
+  static constexpr int kJoin = kWarps * 8 * DP * 4;          // 8 rows of every warp's O
+  static constexpr int kSmem = kRing + kJoin + kWarps * kRows * 2 * 4;
 };
 
-struct Params {
-  const void* q;
-  void* out;
-  float* lse;
-  const void *k, *v;
-  const int *table, *lengths, *prefix_pages;
-  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;
-  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;
-  int64_t table_ld;
-  int B, n, H, Hk, G, D;
-  int num_pages, page_size, table_cols;
-  int prefix;  // keys before the sequences' own, common to all
-  float scale_log2;
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A place on the line of units.
+struct Place {
+  int b, hk, rt;  // item: sequence, K/V head, tile of 16 rows
+  int j, units;   // unit of the item, and how many it has
+  int keys;       // prefix + own keys of the sequence
+  __device__ __forceinline__ void enter(const Params& p) {
+    keys = b < p.B ? p.prefix + own_length(p, b) : 0;
+    units = max(1, (keys + kUnit - 1) / kUnit);
+  }
+  __device__ __forceinline__ void advance(const Params& p, int tiles) {
+    if (++j < units) return;
+    j = 0;
+    if (++rt < tiles) return;
+    rt = 0;
+    if (++hk < p.Hk) return;
+    hk = 0;
+    ++b;
+    enter(p);
+  }
 };
 
-template <bool kBf16>
-__device__ __forceinline__ float to_float(const uint16_t v) {
-  if constexpr (kBf16) return __uint_as_float((uint32_t)v << 16);
-  else return __half2float(__ushort_as_half(v));
-}
-
-__device__ __forceinline__ int sequence_length(const Params& p, int b) {
-  int L = max(0, p.lengths[b]);
-  if ((int64_t)L > (int64_t)p.table_cols * p.page_size) {
-    record_bad_index(kSiteLength);
-    L = p.table_cols * p.page_size;
-  }
-  return L;
-}
-
-// One block per (sequence, token, query head); its warps take every fourth key.
-template <bool kBf16>
-__global__ void __launch_bounds__(128) paged_simple_kernel(const Params p) {
-  const int h = blockIdx.x % p.H, i = blockIdx.x / p.H % p.n, b = blockIdx.x / p.H / p.n;
-  const int hk = h / p.G, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + i * p.q_ss + h * p.q_sh;
-  float qr[4], acc[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-  for (int c = 0; c < 4; ++c) qr[c] = lane + 32 * c < p.D ? to_float<kBf16>(q[lane + 32 * c]) : 0.f;
-  const int seen = max(0, sequence_length(p, b) - p.n + i + 1);
-  for (int j = warp; j < p.prefix + seen; j += 4) {
-    const int t = j < p.prefix ? j : j - p.prefix;
-    int page = (j < p.prefix ? p.prefix_pages : p.table + b * p.table_ld)[t / p.page_size];
-    if (page < 0 || page >= p.num_pages) {
-      record_bad_index(kSitePage);
-      continue;
-    }
-    const int in = t % p.page_size;
-    const uint16_t* k = static_cast<const uint16_t*>(p.k) + page * p.k_sp + in * p.k_ss + hk * p.k_sh;
-    const uint16_t* v = static_cast<const uint16_t*>(p.v) + page * p.v_sp + in * p.v_ss + hk * p.v_sh;
-    float x = 0;
-    for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < p.D) x += qr[c] * to_float<kBf16>(k[lane + 32 * c]);
-    for (int o = 16; o; o /= 2) x += __shfl_xor_sync(~0u, x, o);
-    x *= p.scale_log2;
-    const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top, a = exp2f(m - ref), e = exp2f(x - ref);
-    l = l * a + e;
-    for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < p.D) acc[c] = acc[c] * a + e * to_float<kBf16>(v[lane + 32 * c]);
-    m = top;
-  }
-  __shared__ float sm[4], sl[4], so[4][128];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-  for (int c = 0; c < 4; ++c) so[warp][lane + 32 * c] = acc[c];
+// Units of all items, and the place of unit `first(U)`; every thread gets both.  The lengths are
+// read by the whole block, kThreads at a time.
+template <class First>
+__device__ __forceinline__ Place locate(const Params& p, int per_seq, int tiles, int* sh, int64_t* total, First first) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto units_of = [&](int b) { return b < p.B ? max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) : 0; };
+  long long* sums = reinterpret_cast<long long*>(sh);  // [kWarps] and a result
+  long long mine = 0;
+  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += units_of(b);
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+  if (lane == 0) sums[warp] = mine;
   __syncthreads();
-  float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), sum = 0, o = 0;
-  for (int w = 0; w < 4 && top > -INFINITY; ++w) {
-    const float a = exp2f(sm[w] - top);
-    sum += sl[w] * a;
-    o += so[w][threadIdx.x] * a;
+  long long all = 0;
+  for (int w = 0; w < kWarps; ++w) all += sums[w];
+  *total = all * per_seq;
+  const int64_t u = first(*total);
+  __shared__ int found[3];
+  // The sequence whose units hold u: scan of the lengths, kThreads a step.
+  long long base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int n = units_of(b0 + (int)threadIdx.x);
+    int scan = n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, scan, o);
+      if (lane >= o) scan += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    long long before = base, step = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sums[w];
+      step += sums[w];
+    }
+    const long long lo = (before + scan - n) * per_seq, hi = (before + scan) * per_seq;
+    if (n > 0 && lo <= u && u < hi) {
+      found[0] = b0 + threadIdx.x;
+      found[1] = (int)((u - lo) / n);
+      found[2] = (int)((u - lo) % n);
+    }
+    base += step;
+    if (base * per_seq > u) break;
   }
-  if ((int)threadIdx.x < p.D) {
-    const float r = sum > 0 ? o / sum : 0.f;
-    uint16_t* out = static_cast<uint16_t*>(p.out) + b * p.o_sb + i * p.o_ss + h * p.o_sh;
-    if constexpr (kBf16) reinterpret_cast<__nv_bfloat16*>(out)[threadIdx.x] = __float2bfloat16(r);
-    else reinterpret_cast<__half*>(out)[threadIdx.x] = __float2half(r);
+  __syncthreads();
+  Place at;
+  at.b = found[0];
+  at.hk = found[1] / tiles;
+  at.rt = found[1] % tiles;
+  at.j = found[2];
+  at.enter(p);
+  return at;
+}
+
+template <int DP, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params p) {
+  using C = Cfg<DP>;
+  constexpr int kChunks = DP / 8;          // 16-byte pieces of a row
+  constexpr int kPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* sO = reinterpret_cast<float*>(smem + C::kRing);                // [kWarps][8][DP], swizzled
+  float* sM = reinterpret_cast<float*>(smem + C::kRing + C::kJoin);     // [kWarps][kRows]
+  float* sL = sM + kWarps * kRows;
+  __shared__ int s_last;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = (p.rows + kRows - 1) / kRows;
+  const int per_seq = p.Hk * tiles;
+  Line line;
+  const int c = blockIdx.x;
+  Place at = locate(p, per_seq, tiles, reinterpret_cast<int*>(sM), &line.units, [&](int64_t U) {
+    line.units = U;
+    line.nc = (int)min((int64_t)gridDim.x, U);  // every block that takes part has a unit
+    return c < line.nc ? line.begin(c) : 0;
+  });
+  if (c >= line.nc) return;
+  const int64_t u0 = line.begin(c);
+  const int todo = (int)(line.begin(c + 1) - u0);  // units of this block
+  __syncthreads();
+
+  // ------------------------------------------------------------------ loads
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * C::kTile);
+  const int chunk = lane % kChunks, sub = lane / kChunks;
+  const bool chunk_in = chunk * 8 < p.D;
+  Place ld = at;
+  int ld_left = todo;
+  // Lane l (and l + 16) looks up the page of key l of this warp's group, one step ahead.
+  auto look_up = [&]() {
+    const int t = ld.j * kUnit + warp * kGroup + (lane & 15);
+    if (ld_left <= 0 || t >= ld.keys) return -1;
+    const int o = t - p.prefix;
+    const int page = o < 0 ? p.prefix_pages[t / p.page_size] : p.table[ld.b * p.table_ld + o / p.page_size];
+    if ((unsigned)page >= (unsigned)p.num_pages) {
+      record_bad_index(kSitePage);
+      return -1;
+    }
+    return page;
+  };
+  int page = look_up();
+  int ld_stage = 0;
+  auto load = [&]() {
+    if (ld_left > 0) {
+      const int t = ld.j * kUnit + warp * kGroup + (lane & 15);
+      const int o = t - p.prefix;
+      const int in = (o < 0 ? t : o) % p.page_size;
+      const int64_t ok = page < 0 ? -1 : page * p.k_sp + in * p.k_ss + ld.hk * p.k_sh;
+      const int64_t ov = page < 0 ? -1 : page * p.v_sp + in * p.v_ss + ld.hk * p.v_sh;
+      const uint32_t dst = ring + ld_stage * (2 * C::kTile);
+#pragma unroll
+      for (int i = 0; i < kGroup / kPerCopy; ++i) {
+        const int r = i * kPerCopy + sub;
+        const int64_t rk = __shfl_sync(~0u, ok, r), rv = __shfl_sync(~0u, ov, r);
+        const bool read = rk >= 0 && chunk_in;
+        const uint32_t at_row = r * (DP * 2) + ((chunk ^ (r & 7)) << 4);
+        cp16(dst + at_row, static_cast<const uint16_t*>(p.k) + (read ? rk + chunk * 8 : 0), read);
+        cp16(dst + C::kTile + at_row, static_cast<const uint16_t*>(p.v) + (read ? rv + chunk * 8 : 0), read);
+      }
+      ld.advance(p, tiles);
+      --ld_left;
+      page = look_up();
+      ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load();
+
+  // ------------------------------------------------------------------ items
+  int stage = 0;
+  int64_t unit = u0;
+  const int r0 = lane >> 2;  // this lane's rows: r0 and r0 + 8
+  for (int done = 0; done < todo;) {
+    const int seg = min(at.units - at.j, todo - done);  // units of this item here
+    // Q: row r of the tile is query row rt * 16 + r = token i, head g of the group.
+    uint32_t qf[DP / 16][4];
+    int lim[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = at.rt * kRows + r0 + 8 * h;
+      const bool in = row < p.rows;
+      const int i = in ? row / p.G : 0, g = in ? row - i * p.G : 0;
+      // Keys below lim are seen: the prefix and the own keys up to the token's own.
+      lim[h] = p.prefix + max(0, at.keys - p.prefix - p.n + i + 1);
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + i * p.q_ss +
+                            (int64_t)(at.hk * p.G + g) * p.q_sh + 2 * (lane & 3);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = ks * 16 + 2 * (lane & 3);
+        qf[ks][h] = in && d < p.D ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
+        qf[ks][2 + h] = in && d + 8 < p.D ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
+      }
+    }
+    // Tokens see at least this many keys: units below need no mask.
+    const int all_see = p.prefix + max(0, at.keys - p.prefix - p.n + 1);
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int s = 0; s < seg; ++s) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      load();  // into the stage that the step before this one has read
+      const uint32_t sk = ring + stage * (2 * C::kTile), sv = sk + C::kTile;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      float x[2][4] = {};
+      {
+        // K rows are the B operand's columns: lane l addresses row (l & 7) + 8 (l >> 4) and the
+        // 16-byte piece 2 ks + (l >> 3 & 1).
+        const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          uint32_t kf[4];
+          ldsm4(sk + r * (DP * 2) + (((2 * ks + half) ^ (r & 7)) << 4), kf);
+          mma16816<kBf16>(x[0], qf[ks], kf[0], kf[1]);
+          mma16816<kBf16>(x[1], qf[ks], kf[2], kf[3]);
+        }
+      }
+      const int t0 = (at.j + s) * kUnit + warp * kGroup;
+      if (t0 + kGroup > all_see) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t0 + nt * 8 + 2 * (lane & 3) + (e & 1) >= lim[e >> 1]) x[nt][e] = -INFINITY;
+      }
+      float top[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float t = fmaxf(fmaxf(x[0][2 * h], x[0][2 * h + 1]), fmaxf(x[1][2 * h], x[1][2 * h + 1]));
+        t = fmaxf(t, __shfl_xor_sync(~0u, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
+        top[h] = t * p.scale_log2;
+      }
+      // The maximum in use moves only when it is passed by more than 2^8: P stays below 2^8.
+      if (__any_sync(~0u, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float now = fmaxf(m[h], top[h]);
+          const float a = weight(m[h], now);
+          m[h] = now;
+          l[h] *= a;
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) o[i][2 * h] *= a, o[i][2 * h + 1] *= a;
+        }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float ref = m[h] == -INFINITY ? 0.f : m[h];
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = fa::ex2(fmaf(x[i >> 1][2 * h + (i & 1)], p.scale_log2, -ref));
+        l[h] += (e[0] + e[1]) + (e[2] + e[3]);
+        // P is rounded to the inputs' type for the matrix product; the sum l is of the unrounded.
+        pf[h] = pack2<kBf16>(e[0], e[1]);
+        pf[2 + h] = pack2<kBf16>(e[2], e[3]);
+      }
+      {
+        const int r = lane & 15, half = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          uint32_t vf[4];
+          ldsm4_t(sv + r * (DP * 2) + (((2 * i + half) ^ (r & 7)) << 4), vf);
+          mma16816<kBf16>(o[2 * i], pf, vf[0], vf[1]);
+          mma16816<kBf16>(o[2 * i + 1], pf, vf[2], vf[3]);
+        }
+      }
+      __syncwarp();
+    }
+
+    // ---------------------------------------------------------------- end of the item's share
+    const int64_t item0 = unit - at.j;  // the item's first unit
+    const int cf = line.block_of(item0), cl = line.block_of(item0 + at.units - 1);
+    const bool split = cf != cl;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(~0u, l[h], 1);
+      l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      if ((lane & 3) == 0) {
+        sM[warp * kRows + r0 + 8 * h] = m[h];
+        sL[warp * kRows + r0 + 8 * h] = l[h];
+      }
+    }
+    const int rows_here = min(kRows, p.rows - at.rt * kRows);
+    // Slot of block x's share of a split item: 2 x if it began before x, else 2 x + 1.
+    auto slot_of = [&](int x) { return p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kRows * (DP + 2); };
+    constexpr int kPer = 8 * DP / kThreads;  // values of 8 rows that a thread joins (8 or 4)
+    const int jr = threadIdx.x / (DP / kPer), jd = threadIdx.x % (DP / kPer) * kPer;
+    auto write_out = [&](int row, float mm, float ll, const float (&v)[kPer]) {
+      const int q_row = at.rt * kRows + row;
+      const int i = q_row / p.G, g = q_row - i * p.G, head = at.hk * p.G + g;
+      const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+      if (jd < p.D) {
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + at.b * p.o_sb + i * p.o_ss + head * p.o_sh + jd;
+        uint32_t w[kPer / 2];
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) w[e] = pack2<kBf16>(v[2 * e] * inv, v[2 * e + 1] * inv);
+        if constexpr (kPer == 8)
+          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else
+          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      }
+      if (p.lse && jd == 0)
+        p.lse[((int64_t)at.b * p.n + i) * p.H + head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+    };
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half * 8 >= rows_here) break;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        const int d = i * 8 + 2 * (lane & 3);
+        *reinterpret_cast<float2*>(sO + (warp * 8 + r0) * DP + (d ^ ((r0 & 7) * 8 % DP))) =
+            make_float2(o[i][half ? 2 : 0], o[i][half ? 3 : 1]);
+      }
+      __syncthreads();
+      const int row = half * 8 + jr;
+      if (row < rows_here) {
+        float mw[kWarps], mm = -INFINITY, ll = 0.f, v[kPer] = {};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mw[w] = sM[w * kRows + row], mm = fmaxf(mm, mw[w]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float a = weight(mw[w], mm);
+          ll += a * sL[w * kRows + row];
+          const float* src = sO + (w * 8 + jr) * DP + (jd ^ (jr * 8 % DP));
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) v[e] += a * src[e];
+        }
+        if (!split) {
+          write_out(row, mm, ll, v);
+        } else {
+          float* dst = slot_of(c) + row * (DP + 2);
+          if (jd == 0) dst[DP] = mm, dst[DP + 1] = ll;
+#pragma unroll
+          for (int e = 0; e < kPer; e += 2) *reinterpret_cast<float2*>(dst + jd + e) = make_float2(v[e], v[e + 1]);
+        }
+      }
+      __syncthreads();
+    }
+    if (split) {
+      if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = atomicAdd(&p.counters[cf], 1) == cl - cf;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int half = 0; half < (rows_here + 7) / 8; ++half) {
+          const int row = half * 8 + jr;
+          if (row >= rows_here) continue;
+          float mm = -INFINITY, ll = 0.f, v[kPer] = {};
+          for (int x = cf; x <= cl; ++x) mm = fmaxf(mm, __ldcg(slot_of(x) + row * (DP + 2) + DP));
+          for (int x = cf; x <= cl; ++x) {
+            const float* src = slot_of(x) + row * (DP + 2);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + DP));
+            const float a = weight(ml.x, mm);
+            ll += a * ml.y;
+#pragma unroll
+            for (int e = 0; e < kPer; e += 2) {
+              const float2 f = __ldcg(reinterpret_cast<const float2*>(src + jd + e));
+              v[e] += a * f.x, v[e + 1] += a * f.y;
+            }
+          }
+          write_out(row, mm, ll, v);
+        }
+        if (threadIdx.x == 0) p.counters[cf] = 0;
+      }
+    }
+    // Past this item.
+    done += seg;
+    unit += seg;
+    at.j += seg - 1;
+    at.advance(p, tiles);
   }
-  if (threadIdx.x == 0 && p.lse)
-    p.lse[((int64_t)b * p.n + i) * p.H + h] = sum > 0 ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+  cp_wait<0>();
+}
+
+template <int DP, bool kBf16>
+int launch_rows16(const Params& p, int64_t max_units, cudaStream_t s) {
+  using C = Cfg<DP>;
+  auto kern = paged_rows16_kernel<DP, kBf16>;
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return cuda_status(e);
+    configured.fetch_or(bit);
+  }
+  int64_t grid = 2 * (int64_t)sm_count();
+  if (grid > max_units) grid = max_units;
+  if (grid > kCounters) grid = kCounters;
+  kern<<<(unsigned)grid, kThreads, C::kSmem, s>>>(p);
+  return check_launch();
 }
 
 }  // namespace paged
 }  // namespace lk
 
-extern "C" int64_t lk_paged_attention_workspace_bytes(int64_t H, int64_t H_kv, int64_t D) { return 256; }
+extern "C" int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D) {
+  using namespace lk::paged;
+  if (B < 0 || n < 0 || H < 1 || H_kv < 1 || D < 1) return 0;
+  return kCounters * 4 + (int64_t)4 * lk::sm_count() * kRows * 130 * 4;
+}
 
 extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache,
                                           const int32_t* prefix_pages, int64_t prefix_length, const int32_t* block_table,
@@ -119,15 +479,18 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
     return LK_ERR_INVALID_ARG;
   if (dtype != LK_F16 && dtype != LK_BF16) return LK_ERR_UNSUPPORTED;
   if (D < 8 || D > 128 || D % 8) return LK_ERR_UNSUPPORTED;
-  constexpr int64_t kMax = 1 << 30;
-  if (B > kMax || n > kMax || H > kMax || B * n > kMax / H || num_pages > 0x7FFFFFFF || page_size > kMax ||
-      table_cols > kMax / page_size || prefix_length > kMax)
+  constexpr int64_t kMax = 1 << 30, kMaxKeys = 1 << 29;
+  if (B > kMax || n > kMax || H > kMax || B > kMax / n || B * n > kMax / H || num_pages > 0x7FFFFFFF || page_size > kMax ||
+      table_cols > kMaxKeys / page_size || prefix_length > kMaxKeys)
     return LK_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return LK_ERR_ALIGNMENT;
   for (int i = 0; i < 12; ++i)
     if (strides[i] % 8) return LK_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int st = bind_stream(s)) return st;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < lk_paged_attention_workspace_bytes(B, n, H, H_kv, D))
+    return LK_ERR_INVALID_ARG;
   paged::Params p{};
   p.q = q, p.out = out, p.lse = lse, p.k = k_cache, p.v = v_cache;
   p.table = block_table, p.lengths = lengths, p.prefix_pages = prefix_pages;
@@ -137,12 +500,18 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   p.v_sp = strides[9], p.v_ss = strides[10], p.v_sh = strides[11];
   p.table_ld = table_ld, p.table_cols = (int)table_cols;
   p.B = (int)B, p.n = (int)n, p.H = (int)H, p.Hk = (int)H_kv, p.G = (int)(H / H_kv), p.D = (int)D;
+  p.rows = p.n * p.G;
   p.num_pages = (int)num_pages, p.page_size = (int)page_size, p.prefix = (int)prefix_length;
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = scale * 1.4426950408889634f;
-  if (dtype == LK_BF16) paged::paged_simple_kernel<true><<<(unsigned)(B * n * H), 128, 0, s>>>(p);
-  else paged::paged_simple_kernel<false><<<(unsigned)(B * n * H), 128, 0, s>>>(p);
-  return check_launch();
+  p.counters = static_cast<int*>(workspace);
+  p.partial = reinterpret_cast<float*>(p.counters + paged::kCounters);
+  const bool bf16 = dtype == LK_BF16;
+  const int64_t tiles = (p.rows + paged::kRows - 1) / paged::kRows;
+  const int64_t keys = prefix_length + table_cols * page_size;  // at most
+  const int64_t units = B * H_kv * tiles * (keys > paged::kUnit ? (keys + paged::kUnit - 1) / paged::kUnit : 1);
+  if (D > 64) return bf16 ? paged::launch_rows16<128, true>(p, units, s) : paged::launch_rows16<128, false>(p, units, s);
+  return bf16 ? paged::launch_rows16<64, true>(p, units, s) : paged::launch_rows16<64, false>(p, units, s);
 }
 
 extern "C" int lk_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
