@@ -31,6 +31,8 @@ constexpr int kGroup = 16;             // keys of one warp's step
 constexpr int kUnit = kWarps * kGroup;  // keys of a unit
 constexpr int kStages = 3;
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
+// Units of 64 prefix keys, over all sequences and K/V heads, from which the prefix pass pays.
+constexpr int64_t kPrefixPass = 1024;
 
 template <int DP>
 struct Cfg {
@@ -96,59 +98,6 @@ struct Place {
   }
 };
 
-// Units of all items, and the place of unit `first(U)`; every thread gets both.  The lengths are
-// read by the whole block, kThreads at a time.
-template <class First>
-__device__ __forceinline__ Place locate(const Params& p, int per_seq, int tiles, int* sh, int64_t* total, First first) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto units_of = [&](int b) { return b < p.B ? max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) : 0; };
-  long long* sums = reinterpret_cast<long long*>(sh);  // [kWarps] and a result
-  long long mine = 0;
-  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += units_of(b);
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
-  if (lane == 0) sums[warp] = mine;
-  __syncthreads();
-  long long all = 0;
-  for (int w = 0; w < kWarps; ++w) all += sums[w];
-  *total = all * per_seq;
-  const int64_t u = first(*total);
-  __shared__ int found[3];
-  // The sequence whose units hold u: scan of the lengths, kThreads a step.
-  long long base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int n = units_of(b0 + (int)threadIdx.x);
-    int scan = n;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(~0u, scan, o);
-      if (lane >= o) scan += x;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = scan;
-    __syncthreads();
-    long long before = base, step = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += sums[w];
-      step += sums[w];
-    }
-    const long long lo = (before + scan - n) * per_seq, hi = (before + scan) * per_seq;
-    if (n > 0 && lo <= u && u < hi) {
-      found[0] = b0 + threadIdx.x;
-      found[1] = (int)((u - lo) / n);
-      found[2] = (int)((u - lo) % n);
-    }
-    base += step;
-    if (base * per_seq > u) break;
-  }
-  __syncthreads();
-  Place at;
-  at.b = found[0];
-  at.hk = found[1] / tiles;
-  at.rt = found[1] % tiles;
-  at.j = found[2];
-  at.enter(p);
-  return at;
-}
-
 template <int DP, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params p) {
   using C = Cfg<DP>;
@@ -165,15 +114,24 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const int per_seq = p.Hk * tiles;
   Line line;
   const int c = blockIdx.x;
-  Place at = locate(p, per_seq, tiles, reinterpret_cast<int*>(sM), &line.units, [&](int64_t U) {
-    line.units = U;
-    line.nc = (int)min((int64_t)gridDim.x, U);  // every block that takes part has a unit
-    return c < line.nc ? line.begin(c) : 0;
-  });
+  const Found found = locate<kThreads>(
+      p.B, per_seq, reinterpret_cast<long long*>(sM), &line.units,
+      [&](int b) { return max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit); },
+      [&](int64_t U) {
+        line.units = U;
+        line.nc = (int)min((int64_t)gridDim.x, U);  // every block that takes part has a unit
+        return c < line.nc ? line.begin(c) : 0;
+      });
+  Place at;
+  at.b = found.b;
+  at.enter(p);
+  at.hk = (int)(found.offset / at.units);
+  at.j = (int)(found.offset - (int64_t)at.hk * at.units);
+  at.rt = at.hk % tiles;
+  at.hk /= tiles;
   if (c >= line.nc) return;
   const int64_t u0 = line.begin(c);
   const int todo = (int)(line.begin(c + 1) - u0);  // units of this block
-  __syncthreads();
 
   // ------------------------------------------------------------------ loads
   const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * C::kTile);
@@ -334,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(~0u, l[h], 1);
       l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      if (l[h] != l[h]) m[h] = fmaxf(m[h], 0.f);  // scores that are no numbers stay so when shares are joined
       if ((lane & 3) == 0) {
         sM[warp * kRows + r0 + 8 * h] = m[h];
         sL[warp * kRows + r0 + 8 * h] = l[h];
@@ -344,9 +303,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     auto slot_of = [&](int x) { return p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kRows * (DP + 2); };
     constexpr int kPer = 8 * DP / kThreads;  // values of 8 rows that a thread joins (8 or 4)
     const int jr = threadIdx.x / (DP / kPer), jd = threadIdx.x % (DP / kPer) * kPer;
-    auto write_out = [&](int row, float mm, float ll, const float (&v)[kPer]) {
+    auto write_out = [&](int row, float mm, float ll, float (&v)[kPer]) {
       const int q_row = at.rt * kRows + row;
       const int i = q_row / p.G, g = q_row - i * p.G, head = at.hk * p.G + g;
+      if (p.pre.slots) join_prefix<DP, kPer, 8>(p.pre, p.Hk, at.hk, (int64_t)at.b * p.rows + q_row, jd, mm, ll, v);
       const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
       if (jd < p.D) {
         uint16_t* dst = static_cast<uint16_t*>(p.out) + at.b * p.o_sb + i * p.o_ss + head * p.o_sh + jd;
@@ -361,6 +321,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
       if (p.lse && jd == 0)
         p.lse[((int64_t)at.b * p.n + i) * p.H + head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
     };
+#pragma unroll
+    if (p.pre.slots) griddep_wait();  // the prefix's shares are complete
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half * 8 >= rows_here) break;
@@ -387,10 +349,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
         if (!split) {
           write_out(row, mm, ll, v);
         } else {
-          float* dst = slot_of(c) + row * (DP + 2);
-          if (jd == 0) dst[DP] = mm, dst[DP + 1] = ll;
+          float* dst = slot_of(c);
+          if (jd == 0) *reinterpret_cast<float2*>(dst + kRows * DP + 2 * row) = make_float2(mm, ll);
 #pragma unroll
-          for (int e = 0; e < kPer; e += 2) *reinterpret_cast<float2*>(dst + jd + e) = make_float2(v[e], v[e + 1]);
+          for (int e = 0; e < kPer; e += 4)
+            *reinterpret_cast<float4*>(dst + row * DP + jd + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         }
       }
       __syncthreads();
@@ -407,18 +370,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
           const int row = half * 8 + jr;
           if (row >= rows_here) continue;
           float mm = -INFINITY, ll = 0.f, v[kPer] = {};
-          for (int x = cf; x <= cl; ++x) mm = fmaxf(mm, __ldcg(slot_of(x) + row * (DP + 2) + DP));
-          for (int x = cf; x <= cl; ++x) {
-            const float* src = slot_of(x) + row * (DP + 2);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + DP));
-            const float a = weight(ml.x, mm);
-            ll += a * ml.y;
-#pragma unroll
-            for (int e = 0; e < kPer; e += 2) {
-              const float2 f = __ldcg(reinterpret_cast<const float2*>(src + jd + e));
-              v[e] += a * f.x, v[e + 1] += a * f.y;
-            }
-          }
+          join_shares<DP, kPer, 8>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, row, jd, mm, ll, v);
           write_out(row, mm, ll, v);
         }
         if (threadIdx.x == 0) p.counters[cf] = 0;
@@ -449,17 +401,49 @@ int launch_rows16(const Params& p, int64_t max_units, cudaStream_t s) {
   int64_t grid = 2 * (int64_t)sm_count();
   if (grid > max_units) grid = max_units;
   if (grid > kCounters) grid = kCounters;
-  kern<<<(unsigned)grid, kThreads, C::kSmem, s>>>(p);
-  return check_launch();
+  return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.pre.slots != nullptr, s, p);
 }
 
 }  // namespace paged
 }  // namespace lk
 
-extern "C" int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D) {
+namespace lk {
+namespace paged {
+namespace {
+// How the prefix pass cuts its work (paged_common.cuh); slots is left to the caller.
+PrefixShares prefix_shares(int64_t rows, int64_t H_kv, int64_t prefix) {
+  PrefixShares s{};
+  const int sms = sm_count();
+  s.tile = rows <= kWideRows / 2 ? kWideRows / 2 : kWideRows;
+  s.pairs = (int)((rows + s.tile - 1) / s.tile);
+  s.units = (int)((prefix + 127) / 128);
+  // The pairs of a K/V head go side by side where that leaves at most a seventh of the SMs idle.
+  s.lines = s.pairs <= sms && sms / s.pairs * s.pairs * 7 >= sms * 6 ? s.pairs : 1;
+  const int64_t items = s.lines > 1 ? H_kv : H_kv * s.pairs;
+  s.nc = sms / s.lines;
+  if (s.nc > items * s.units) s.nc = (int)(items * s.units);
+  return s;
+}
+int64_t prefix_floats(const PrefixShares& s, int64_t H_kv, int64_t DP) {
+  const int64_t items = s.lines > 1 ? H_kv : H_kv * s.pairs;
+  return s.lines * (items + s.nc) * kWideRows * (DP + 2);
+}
+// Floats of the shares of sequences' own keys.
+int64_t own_floats(int64_t rows, int64_t DP) {
+  return rows > kRows ? (int64_t)2 * sm_count() * kWideRows * (DP + 2) : (int64_t)4 * sm_count() * kRows * (DP + 2);
+}
+}  // namespace
+}  // namespace paged
+}  // namespace lk
+
+extern "C" int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D,
+                                                      int64_t prefix_length) {
   using namespace lk::paged;
-  if (B < 0 || n < 0 || H < 1 || H_kv < 1 || D < 1) return 0;
-  return kCounters * 4 + (int64_t)4 * lk::sm_count() * kRows * 130 * 4;
+  if (B < 1 || n < 1 || H < 1 || H_kv < 1 || D < 1 || prefix_length < 0) return 0;
+  const int64_t DP = D > 64 ? 128 : 64, rows = n * (H / H_kv);
+  int64_t floats = kCounters + own_floats(rows, DP);
+  if (prefix_length > 0) floats += prefix_floats(prefix_shares(B * rows, H_kv, prefix_length), H_kv, DP);
+  return (floats * 4 + 255) / 256 * 256;
 }
 
 extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -489,7 +473,7 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int st = bind_stream(s)) return st;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-      workspace_bytes < lk_paged_attention_workspace_bytes(B, n, H, H_kv, D))
+      workspace_bytes < lk_paged_attention_workspace_bytes(B, n, H, H_kv, D, prefix_length))
     return LK_ERR_INVALID_ARG;
   paged::Params p{};
   p.q = q, p.out = out, p.lse = lse, p.k = k_cache, p.v = v_cache;
@@ -507,9 +491,21 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   p.counters = static_cast<int*>(workspace);
   p.partial = reinterpret_cast<float*>(p.counters + paged::kCounters);
   const bool bf16 = dtype == LK_BF16;
-  const int64_t tiles = (p.rows + paged::kRows - 1) / paged::kRows;
-  const int64_t keys = prefix_length + table_cols * page_size;  // at most
-  const int64_t units = B * H_kv * tiles * (keys > paged::kUnit ? (keys + paged::kUnit - 1) / paged::kUnit : 1);
+  const int64_t DP = D > 64 ? 128 : 64;
+  bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
+  for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
+  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
+    paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
+    pre.slots = p.partial + paged::own_floats(p.rows, DP);
+    p.pre = pre;
+    if (int st = paged::launch_wide(p, bf16, true, 0, s)) return st;
+    p.prefix = 0;
+  }
+  const int64_t keys = p.prefix + table_cols * page_size;  // at most
+  auto at_most = [&](int64_t items, int64_t unit) { return items * (keys > unit ? (keys + unit - 1) / unit : 1); };
+  if (p.rows > paged::kRows && wide && p.prefix == 0)
+    return paged::launch_wide(p, bf16, false, at_most(B * H_kv * ((p.rows + 127) / 128), 128), s);
+  const int64_t units = at_most(B * H_kv * ((p.rows + paged::kRows - 1) / paged::kRows), paged::kUnit);
   if (D > 64) return bf16 ? paged::launch_rows16<128, true>(p, units, s) : paged::launch_rows16<128, false>(p, units, s);
   return bf16 ? paged::launch_rows16<64, true>(p, units, s) : paged::launch_rows16<64, false>(p, units, s);
 }

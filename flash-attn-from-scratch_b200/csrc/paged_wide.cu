@@ -1,0 +1,853 @@
+// paged_wide.cu — attention over a paged key/value cache for many query rows per K/V head, on
+// the tensor cores: tcgen05 MMAs into tensor memory, K/V pages streamed by TMA.
+//
+// Two uses of one kernel.  The prefix pass: all the batch's queries of a K/V head against the
+// keys that the sequences share, read once for 256 rows; it leaves (m, l, o) shares that the
+// kernel over the sequences' own keys joins.  And sequences with more than 16 query rows per
+// K/V head (pieces of prompts, many drafted tokens, one K/V head for many query heads).
+//
+// Bound: with 256 rows a block does 256 flops per byte of K/V, near the card's balance (~250), so
+// both matter: the tensor pipe runs S = Q K^T and O += P V of two 128-row tiles in turn while
+// eight softmax warps (a thread = a row) work on the other tile's exponentials, and TMA streams
+// pages through a ring.  The roles and the tensor-memory layout are those of the flash-attention
+// forward kernel (flash_attn.cu):
+//   warps 0-3, 4-7  softmax of tile 0, 1; they also gather the rows of Q (any stride, any group
+//                   size) into swizzled shared memory, and write or share the results
+//   warp 8          TMA producer: K_0, V_0, K_1, V_1, ... of 128 keys, page by page: a box is the
+//                   largest power of two of rows that divides the page (8 to 128), a lane each
+//   warp 9          tensor memory and MMA issue
+// A block walks its share of the line of units (paged_common.cuh; a unit is 128 keys) through as
+// many items as that holds; the barriers' phases run on across items.
+//
+// With no more than 128 rows the second tile would idle and S -> softmax -> PV would be one
+// serial chain; there tile 1 takes the same queries over every second key block (two halves of
+// the keys, joined at the item's end: the two tiles' warps see the same lanes of tensor memory).
+//
+// Keys behind a sequence's last one: whole boxes of them are not read (an out-of-range page
+// coordinate gives zeros); in the box that holds the end the rows of V behind it are zeroed in
+// shared memory before the MMA may see them (0 x NaN), and S is masked.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "lk_abi.h"
+#include "paged_common.cuh"
+
+namespace lk {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kTileM = 128;
+constexpr int kBlockN = 128;  // keys of a unit
+constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
+
+enum WideSite : int {
+  kSiteEmpty = 321,
+  kSiteQ = 322,
+  kSiteKV = 323,
+  kSiteP = 324,
+  kSiteS = 325,
+  kSiteO = 326,
+  kSiteFix = 327,
+  kSiteMeet = 328,
+  kSiteTeardown = 329,
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int kBoxes = D / 64;              // 128-byte columns of a row
+  static constexpr int kTile = kTileM * D * 2;       // bytes of a tile of Q, K or V
+  static constexpr int kFit = (232448 - 1024 - 1024 - 2 * kTile) / kTile;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;  // 5 (D = 128), 8 (D = 64)
+  static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 1024;
+  static constexpr int kOCol = 256;
+};
+
+struct WideParams {
+  Params p;
+  int prefix_pass;
+  int64_t rows;    // query rows of an item's (sequence, K/V head); prefix pass: of the K/V head
+  int pairs;       // tiles of 256 (halves == 2: 128) rows
+  int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
+  int box_rows;    // rows of a page in one TMA box
+  int lines;       // prefix pass: lines of units (paged_common.cuh)
+};
+
+// An item's share of a block: blocks [j0, j1) of 128 keys of item (b, hk, pair).
+struct Item {
+  int b, hk, pair;
+  int units;    // key blocks of the item
+  int keys;     // keys that lie in the pages
+  int visible;  // keys that its last row sees
+};
+
+// Where a softmax warp stands on its block's share.  Kept in shared memory: the softmax loop
+// needs its registers for a row of S.
+struct Walk {
+  Item it;
+  int j0, done, todo, c, line_id, item, nc;
+  int64_t unit, units;
+};
+
+__device__ __forceinline__ int visible_keys(const WideParams& w, int L, int pair) {
+  if (w.prefix_pass) return L;
+  const int64_t tile = w.halves == 2 ? kTileM : 2 * kTileM;
+  const int64_t last_row = min(w.rows, (pair + 1) * tile) - 1;
+  const int i = (int)(last_row / w.p.G);
+  return max(0, L - w.p.n + i + 1);
+}
+__device__ __forceinline__ int units_of_keys(int keys) { return max(1, (keys + kBlockN - 1) / kBlockN); }
+
+__device__ __forceinline__ void enter(const WideParams& w, Item& it) {
+  it.visible = visible_keys(w, it.keys, it.pair);
+  it.units = units_of_keys(it.visible);
+}
+// The item behind `it` on the block's line.
+__device__ __forceinline__ void next_item(const WideParams& w, Item& it) {
+  if (w.prefix_pass) {
+    if (w.lines > 1) {
+      ++it.hk;
+    } else if (++it.pair == w.pairs) {
+      it.pair = 0;
+      ++it.hk;
+    }
+    return;  // all items have the prefix's units
+  }
+  if (++it.pair == w.pairs) {
+    it.pair = 0;
+    if (++it.hk == w.p.Hk) {
+      it.hk = 0;
+      ++it.b;
+      it.keys = it.b < w.p.B ? own_length(w.p, it.b) : 0;
+    }
+  }
+  enter(w, it);
+}
+
+// Query row `row` of the item: its sequence, token and head.
+struct Row {
+  int b, i, head;
+};
+__device__ __forceinline__ Row query_row(const WideParams& w, const Item& it, int64_t row) {
+  Row r;
+  if (w.prefix_pass) {
+    const int per = w.p.rows;  // rows of a sequence
+    r.b = (int)(row / per);
+    row -= (int64_t)r.b * per;
+  } else {
+    r.b = it.b;
+  }
+  r.i = (int)(row / w.p.G);
+  r.head = it.hk * w.p.G + (int)(row - (int64_t)r.i * w.p.G);
+  return r;
+}
+
+// Max of n fp32 values (bit patterns), four chains of three-input max.
+template <int n>
+__device__ __forceinline__ float row_max(const uint32_t (&sr)[n]) {
+  float m[4] = {__uint_as_float(sr[0]), __uint_as_float(sr[1]), __uint_as_float(sr[2]), __uint_as_float(sr[3])};
+#pragma unroll
+  for (int c = 4; c < n - 4; c += 8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = max3(m[e], __uint_as_float(sr[c + 2 * e]), __uint_as_float(sr[c + 2 * e + 1]));
+  }
+  m[0] = max3(m[0], __uint_as_float(sr[n - 4]), __uint_as_float(sr[n - 3]));
+  m[1] = max3(m[1], __uint_as_float(sr[n - 2]), __uint_as_float(sr[n - 1]));
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WideParams w) {
+  using C = Cfg<D>;
+  constexpr int S = C::kStages;
+  constexpr uint32_t kIdescS = make_idesc(1, kBf16 ? 1 : 0, kBf16 ? 1 : 0, 0, 0, kTileM, kBlockN);
+  constexpr uint32_t kIdescO = make_idesc(1, kBf16 ? 1 : 0, kBf16 ? 1 : 0, 0, 1, kTileM, D);
+  const Params& p = w.p;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                  // [2][kTile]
+  uint8_t* sRing = smem + 2 * C::kTile;  // [S][kTile]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRing + S * C::kTile);
+  uint64_t* q_full = bars;           // [2]  the softmax warps of tile t have written Q_t
+  uint64_t* kv_full = q_full + 2;    // [S]
+  uint64_t* kv_empty = kv_full + S;  // [S]
+  uint64_t* s_full = kv_empty + S;   // [2]  S_t in TMEM, PV_t of the block before complete
+  uint64_t* p_half = s_full + 2;     // [2]  keys 0-63 of P_t in TMEM, O_t rescaled
+  uint64_t* p_full = p_half + 2;     // [2]  all of P_t
+  uint64_t* o_full = p_full + 2;     // [2]  the item's last PV_t complete
+  uint64_t* fix = o_full + 2;        // [1]  a V tile that needs zeros has landed
+  uint64_t* meet_bar = fix + 1;      // [1]  the eight softmax warps meet
+  uint64_t* drain = meet_bar + 1;    // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* s_last = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile Walk* walks = reinterpret_cast<volatile Walk*>(s_last + 1);  // [8] of the softmax warps
+  long long* scratch = reinterpret_cast<long long*>(sQ);  // before the pipeline starts
+
+  const int warp = warp_id();
+  const int lane = threadIdx.x & 31;
+  griddep_launch_dependents();
+
+  // ------------------------------------------------------------------ this block's share
+  Line line;
+  Item first;
+  int c, line_id = 0;
+  int64_t u0;
+  int j_first;
+  if (w.prefix_pass) {
+    line_id = w.lines > 1 ? (int)blockIdx.x % w.lines : 0;
+    c = w.lines > 1 ? (int)blockIdx.x / w.lines : (int)blockIdx.x;
+    line.nc = gridDim.x / w.lines;
+    first.keys = p.prefix;
+    first.visible = p.prefix;
+    first.units = units_of_keys(p.prefix);
+    line.units = (int64_t)first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs);
+    u0 = line.begin(c);
+    const int item = (int)(u0 / first.units);
+    j_first = (int)(u0 - (int64_t)item * first.units);
+    first.b = 0;
+    first.hk = w.lines > 1 ? item : item / w.pairs;
+    first.pair = w.lines > 1 ? line_id : item % w.pairs;
+  } else {
+    c = blockIdx.x;
+    const Found found = locate<kThreads>(
+        p.B, p.Hk, scratch, &line.units,
+        [&](int b) {
+          const int L = own_length(p, b);
+          int sum = 0;
+          for (int x = 0; x < w.pairs; ++x) sum += units_of_keys(visible_keys(w, L, x));
+          return sum;
+        },
+        [&](int64_t U) {
+          line.units = U;
+          line.nc = (int)min((int64_t)gridDim.x, U);
+          return c < line.nc ? line.begin(c) : 0;
+        });
+    if (c >= line.nc) return;
+    u0 = line.begin(c);
+    first.b = found.b;
+    first.keys = own_length(p, first.b);
+    int per_head = 0;
+    for (int x = 0; x < w.pairs; ++x) per_head += units_of_keys(visible_keys(w, first.keys, x));
+    first.hk = (int)(found.offset / per_head);
+    j_first = (int)(found.offset - (int64_t)first.hk * per_head);
+    first.pair = 0;
+    enter(w, first);
+    while (j_first >= first.units) {
+      j_first -= first.units;
+      ++first.pair;
+      enter(w, first);
+    }
+  }
+  const int todo = (int)(line.begin(c + 1) - u0);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 4);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(fix, 1);
+    mbar_init(meet_bar, 8);
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Key blocks of the item's share [j0, j1) that tile t takes: from `from` to `to` in steps of
+  // `halves` (none where from >= to).
+  const int step = w.halves;
+  auto tile_rows_begin = [&](const Item& it, int t) {
+    return step == 2 ? (int64_t)it.pair * kTileM : ((int64_t)it.pair * 2 + t) * kTileM;  // first row of tile t
+  };
+  auto tile_units = [&](const Item& it, int t) {  // key blocks that tile t's last row sees, at least one
+    const int64_t begin = tile_rows_begin(it, t);
+    if (begin >= w.rows) return 0;
+    if (w.prefix_pass) return it.units;
+    const int i = (int)((min(w.rows, begin + kTileM) - 1) / p.G);
+    return units_of_keys(max(0, it.keys - p.n + i + 1));
+  };
+  auto tile_range = [&](const Item& it, int t, int j0, int j1, int& from, int& to) {
+    from = step == 2 ? j0 + ((j0 ^ t) & 1) : j0;
+    to = min(j1, tile_units(it, t));
+  };
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- TMA producer
+    bool ok = true;
+    int issued = 0, fixes = 0;
+    Item it = first;
+    int j = j_first;
+    const int box = w.box_rows, boxes = kBlockN / box;
+    // Lane g has box g of a block: its page (-1: behind the last key) and the row in it.  Looked
+    // up a block ahead, and not looked at before its turn: the load takes longer than an issue.
+    auto look_up = [&](int& in) {
+      const int t = j * kBlockN + lane * box;
+      in = 0;
+      if (lane >= boxes || t >= it.keys) return -1;
+      const int col = t / p.page_size;
+      in = t - col * p.page_size;
+      return w.prefix_pass ? p.prefix_pages[col] : p.table[it.b * p.table_ld + col];
+    };
+    int in_next, page_next = look_up(in_next);
+    for (int done = 0; done < todo && ok; ++done) {
+      const int in = in_next, hk = it.hk, t = j * kBlockN + lane * box;
+      int page = page_next;
+      const bool held = lane < boxes && t < it.keys;
+      // Keys of the block that the sequence has; the box that holds its end is partly not its.
+      const int have = it.keys - j * kBlockN;
+      const bool ragged = have < kBlockN && have > 0 && have % box != 0;
+      if (++j == it.units && done + 1 < todo) {
+        next_item(w, it);
+        j = 0;
+      }
+      if (done + 1 < todo) page_next = look_up(in_next);
+      if ((unsigned)page >= (unsigned)p.num_pages) {
+        if (held) record_bad_index(kSitePage);
+        page = p.num_pages;  // out of range: zeros
+      }
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        const int slot = issued % S;
+        if (!mbar_wait_warp(&kv_empty[slot], ((issued / S) & 1) ^ 1u, kSiteEmpty)) {
+          ok = false;
+          break;
+        }
+        const bool mend = kv == 1 && ragged;
+        uint64_t* bar = mend ? fix : &kv_full[slot];
+        uint8_t* dst = sRing + slot * C::kTile;
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+        __syncwarp();
+        if (lane < boxes) {
+          const CUtensorMap* tm = kv ? &tmV : &tmK;
+#pragma unroll
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_4d(dst + x * (kTileM * 128) + lane * box * 128, tm, bar, 64 * x, in, hk, page);
+        }
+        ++issued;
+        if (mend) {
+          ok = __all_sync(0xffffffffu, mbar_wait_drain(fix, fixes & 1, kSiteFix));
+          ++fixes;
+          const int end = (have + box - 1) / box * box;
+          for (int i = lane; i < (end - have) * C::kBoxes * 8; i += 32) {
+            const int r = have + i / (C::kBoxes * 8), piece = i % (C::kBoxes * 8);
+            *reinterpret_cast<uint4*>(dst + (piece >> 3) * (kTileM * 128) + r * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[slot]);
+          if (!ok) break;
+        }
+      }
+    }
+    // Every copy issued must land before the block can exit.
+    for (int i = (issued > S ? issued - S : 0); i < issued; ++i)
+      mbar_wait_drain(&kv_full[i % S], (i / S) & 1, kSiteTeardown);
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMA issuer (whole warp)
+    bool ok = true;
+    const uint64_t q_desc[2] = {sdesc_sw128(smem_u32(sQ), 16, 1024),
+                                step == 2 ? sdesc_sw128(smem_u32(sQ), 16, 1024)
+                                          : sdesc_sw128(smem_u32(sQ + C::kTile), 16, 1024)};
+    const uint64_t ring_k = sdesc_sw128(smem_u32(sRing), 16, 1024);
+    const uint64_t ring_v = sdesc_sw128(smem_u32(sRing), kTileM * 128, 1024);
+    int base = 0;           // ring item of the share's first K
+    int cnt[2] = {0, 0};    // blocks done by tile t
+    int q_cnt[2] = {0, 0};  // items whose Q_t has been waited for
+    auto wait_item = [&](int i) {
+      const bool r = mbar_wait_warp(&kv_full[i % S], (i / S) & 1, kSiteKV);
+      tc_fence_after();
+      return r;
+    };
+    auto issue_s = [&](int t, int i) {
+      const uint64_t kd = sdesc_add(ring_k, (i % S) * C::kTile);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t off = (ks >> 2) * (kTileM * 128) + (ks & 3) * 32;
+        mma_f16_ss_warp(tmem + t * kBlockN, sdesc_add(q_desc[t], off), sdesc_add(kd, off), kIdescS, ks > 0);
+      }
+      tc_commit_warp(&s_full[t]);
+    };
+    auto issue_pv = [&](int t, int i, int ks0, int ks1, bool add) {
+      const uint64_t vd = sdesc_add(ring_v, (i % S) * C::kTile);
+#pragma unroll
+      for (int ks = ks0; ks < ks1; ++ks)
+        mma_f16_ts_warp(tmem + C::kOCol + t * D, tmem + t * kBlockN + ks * 8, sdesc_add(vd, ks * 16 * 128), kIdescO,
+                        (add || ks > 0) ? 1u : 0u);
+    };
+    Item it = first;
+    int j0 = j_first;
+    for (int done = 0; done < todo && ok;) {
+      const int seg = min(it.units - j0, todo - done);
+      int from[2], to[2];
+      for (int t = 0; t < 2; ++t) tile_range(it, t, j0, j0 + seg, from[t], to[t]);
+      // Ring item of K_j: base + 2 (j - j0); of V_j: one more.
+      auto k_item = [&](int j) { return base + 2 * (j - j0); };
+      // Q_t is in (its softmax warps write it once the item before is done with it).
+      for (int t = 0; t < 2 && ok; ++t)
+        if (step == 2 ? t == 0 : from[t] < to[t]) ok = mbar_wait_warp(&q_full[t], q_cnt[t]++ & 1, kSiteQ);
+      tc_fence_after();
+      // K_j is waited for once and released once the last tile that takes it has issued.
+      int k_waited = j0 - 1;
+      auto need_k = [&](int j) {
+        while (ok && k_waited < j) ok = wait_item(k_item(++k_waited));
+        return ok;
+      };
+      int k_released = j0 - 1;
+      auto release_k = [&](int j) {
+        while (k_released < j) {
+          ++k_released;
+          tc_commit_warp(&kv_empty[k_item(k_released) % S]);
+        }
+      };
+      for (int t = 0; t < 2 && ok; ++t)
+        if (from[t] < to[t] && need_k(from[t])) issue_s(t, k_item(from[t]));
+      if (ok) release_k(min(j0 + seg - 1, j0 + step - 1));
+      for (int j = j0; j < j0 + seg && ok; ++j) {
+        bool v_in = false;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j < from[t] || j >= to[t] || (step == 2 && ((j ^ from[t]) & 1))) continue;
+          if (!v_in) {
+            if (!(ok = wait_item(k_item(j) + 1))) break;
+            v_in = true;
+          }
+          const bool add = j > from[t];
+          if (!(ok = mbar_wait_warp(&p_half[t], cnt[t] & 1, kSiteP))) break;
+          tc_fence_after();
+          issue_pv(t, k_item(j) + 1, 0, kBlockN / 32, add);
+          if (!(ok = mbar_wait_warp(&p_full[t], cnt[t] & 1, kSiteP))) break;
+          tc_fence_after();
+          issue_pv(t, k_item(j) + 1, kBlockN / 32, kBlockN / 16, add);
+          ++cnt[t];
+          if (j + step < to[t]) {
+            if (!need_k(j + step)) break;
+            issue_s(t, k_item(j + step));
+          } else {
+            tc_commit_warp(&o_full[t]);
+          }
+        }
+        if (!ok) break;
+        if (!v_in) ok = wait_item(k_item(j) + 1);  // no tile takes V_j: its slot is free again
+        if (!ok) break;
+        tc_commit_warp(&kv_empty[(k_item(j) + 1) % S]);
+        const int k_next = min(j + step, j0 + seg - 1);
+        if (!need_k(k_next)) break;
+        release_k(k_next);
+      }
+      base += 2 * seg;
+      done += seg;
+      j0 = 0;
+      if (done < todo) next_item(w, it);
+    }
+    tc_commit_warp(drain);
+    mbar_wait_drain(drain, 0, kSiteTeardown);
+  } else {
+    // ---------------------------------------------------------------- softmax (warps 0-7)
+    const int t = warp >> 2, quad = warp & 3;
+    const int r = quad * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t s_tmem = tmem + lane_off + t * kBlockN;
+    const uint32_t o_tmem = tmem + lane_off + C::kOCol + t * D;
+    bool ok = true;
+    int cnt = 0, o_cnt = 0, meets = 0;
+    auto meet = [&]() {  // a bounded barrier of the softmax warps
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet_bar);
+      return mbar_wait_warp(meet_bar, meets++ & 1, kSiteMeet);
+    };
+    volatile Walk* walk = walks + warp;
+    if (lane == 0) {
+      walk->it.b = first.b, walk->it.hk = first.hk, walk->it.pair = first.pair;
+      walk->it.units = first.units, walk->it.keys = first.keys, walk->it.visible = first.visible;
+      walk->j0 = j_first, walk->done = 0, walk->todo = todo, walk->c = c, walk->line_id = line_id, walk->nc = line.nc;
+      walk->item = !w.prefix_pass ? 0 : (w.lines > 1 ? first.hk : first.hk * w.pairs + first.pair);
+      walk->unit = u0, walk->units = line.units;
+    }
+    __syncwarp();
+    auto item_now = [&]() {
+      Item i;
+      i.b = walk->it.b, i.hk = walk->it.hk, i.pair = walk->it.pair;
+      i.units = walk->it.units, i.keys = walk->it.keys, i.visible = walk->it.visible;
+      return i;
+    };
+    // Row r of the tile, columns 32 x .. 32 x + 31 in 32 bits, in this warp's own rows of the
+    // tile's Q buffer (128-byte swizzle): O's way from a thread per row to whole rows.
+    auto stage_at = [&](int row, int col) {
+      return reinterpret_cast<float4*>(sQ + t * C::kTile + (col >> 5) * (kTileM * 128) + row * 128 +
+                                       ((((col >> 2) & 7) ^ (row & 7)) << 4));
+    };
+    while (ok && walk->done < walk->todo) {
+      int from, to, lim, tile_sees;
+      bool warp_live;
+      {
+        const Item it = item_now();
+        const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done);
+        tile_range(it, t, j0, j0 + seg, from, to);
+        const int64_t row_begin = tile_rows_begin(it, t), row = row_begin + r;
+        const bool live = row < w.rows;
+        warp_live = row_begin + quad * 32 < w.rows;
+        const Row at = query_row(w, it, live ? row : 0);
+        // Keys that this row sees, and that every row of the tile does.
+        lim = !live ? 0 : (w.prefix_pass ? it.keys : max(0, it.keys - p.n + at.i + 1));
+        tile_sees = w.prefix_pass ? it.keys : max(0, it.keys - p.n + 1 + (int)(min(row_begin, w.rows - 1) / p.G));
+        // Q_t is written for every share that its MMAs take part in.  (With two halves both tiles
+        // read Q_0, and the halves meet at the end of each item, so it is idle here.)
+        if (step == 2 ? t == 0 : from < to) {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at.b * p.q_sb +
+                                                            at.i * p.q_ss + at.head * p.q_sh);
+          uint8_t* dst = sQ + t * C::kTile + r * 128;
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            const uint4 v = live && x * 8 < p.D ? src[x] : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dst + (x >> 3) * (kTileM * 128) + (((x & 7) ^ (r & 7)) << 4)) = v;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[t]);
+        }
+      }
+      const bool any = from < to;
+      float m_used = -INFINITY, l = 0.f;
+      bool begun = false;
+#pragma unroll 1
+      for (int j = from; j < to; j += step) {
+        if (!mbar_wait_warp(&s_full[t], cnt & 1, kSiteS)) {
+          ok = false;
+          break;
+        }
+        ++cnt;
+        tc_fence_after();
+        if (!warp_live) {  // no query in this warp's rows: what P holds there reaches no result
+          if (lane == 0) {
+            mbar_arrive(&p_half[t]);
+            mbar_arrive(&p_full[t]);
+          }
+          continue;
+        }
+        uint32_t sr[kBlockN];
+        const int n0 = j * kBlockN;
+#pragma unroll
+        for (int x = 0; x < kBlockN / 32; ++x) tmem_ld32(s_tmem + x * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
+        tmem_wait_ld();
+        if (n0 + kBlockN > tile_sees && n0 + kBlockN > lim) {
+#pragma unroll
+          for (int x = 0; x < kBlockN; ++x)
+            if (n0 + x >= lim) sr[x] = __float_as_uint(-INFINITY);
+        }
+        const float m_new = row_max<kBlockN>(sr) * p.scale_log2;
+        const bool need = m_new > m_used + kLazy;
+        const bool warp_rescale = __any_sync(0xffffffffu, need) && begun;
+        begun = true;
+        float alpha = 1.f;
+        if (need) {
+          alpha = fa::ex2(m_used - m_new);  // 0 where m_used is -inf
+          m_used = m_new;
+        }
+        l *= alpha;
+        const float ref = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
+        const uint64_t ng2 = f2(-ref, -ref);
+        uint64_t rs2 = f2(0.f, 0.f);
+        uint32_t pk[kBlockN / 2];
+#pragma unroll
+        for (int e = 0; e < kBlockN / 2; ++e) {
+          const uint64_t x2 = fma2(f2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, ng2);
+          float x0, x1, p0, p1;
+          uf2(x2, x0, x1);
+          if ((e & 7) == 0) {
+            fa::exp2_poly_pair(x0, x1, p0, p1);
+          } else {
+            p0 = fa::ex2(x0);
+            p1 = fa::ex2(x1);
+          }
+          rs2 = add2(rs2, f2(p0, p1));
+          pk[e] = pack2<kBf16>(p0, p1);  // rounded for the matrix product; the sum is of the unrounded
+          if (e == kBlockN / 4 - 1) {
+            tmem_st32(s_tmem, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+            if (warp_rescale) {
+#pragma unroll 1
+              for (int x = 0; x < D / 32; ++x) {
+                uint32_t ov[32];
+                tmem_ld32(o_tmem + x * 32, ov);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                tmem_st32(o_tmem + x * 32, ov);
+              }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[t]);
+          }
+        }
+        float rs0, rs1;
+        uf2(rs2, rs0, rs1);
+        l += rs0 + rs1;
+        tmem_st32(s_tmem + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      if (any) {
+        if (!(ok = mbar_wait_warp(&o_full[t], o_cnt & 1, kSiteO))) break;
+        ++o_cnt;
+        tc_fence_after();
+      }
+      // A row that saw no key has m = -inf (its l is of the 2^-125 that the polynomial gives for
+      // a masked key); one whose scores were not numbers keeps that.
+      if (l != l) m_used = fmaxf(m_used, 0.f);
+      if (m_used == -INFINITY) l = 0.f;
+
+      // ------------------------------------------------------------ results of the share
+      const Item it = item_now();
+      const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done), item = walk->item;
+      Line ln;
+      ln.nc = walk->nc, ln.units = walk->units;
+      const int64_t item0 = walk->unit - j0;
+      const int me = walk->c, cf = ln.block_of(item0), cl = ln.block_of(item0 + it.units - 1);
+      // A whole item is written at once; a part of one, and what a prefix's shares join, is left
+      // as a share in the workspace.
+      const bool direct = !w.prefix_pass && cf == cl && !p.pre.slots;
+      const int64_t row_begin = tile_rows_begin(it, step == 2 ? 0 : t);
+      const int quad_rows = (int)max((int64_t)0, min((int64_t)32, w.rows - row_begin - quad * 32));  // queries among this warp's rows
+      auto slot_of = [&](int x) {
+        return w.prefix_pass ? prefix_slot<D>(p.pre, p.Hk, walk->line_id, item, x)
+                             : p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kSlotFloats<D>;
+      };
+      // Columns [c0, c1) of O are this warp's to hand on.  With two halves the tiles' warps read
+      // both O_0 and O_1 (the same TMEM lanes) and take half of the columns each.
+      const int c0 = step == 2 ? t * (D / 2) : 0, c1 = step == 2 ? c0 + D / 2 : D;
+      float m_row = m_used, l_row = l, w0 = 1.f, w1 = 0.f;
+      bool any0 = t == 0 && any, any1 = t == 1 && any;
+      if (step == 2) {
+        uint32_t ml[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) ml[i] = 0;
+        ml[0] = __float_as_uint(m_used), ml[1] = __float_as_uint(l);
+        tmem_st32(s_tmem, ml);  // S_t is idle: every MMA of the item is complete
+        tmem_wait_st();
+        tc_fence_before();
+        if (!(ok = meet())) break;
+        tc_fence_after();
+        tmem_ld32(tmem + lane_off + (1 - t) * kBlockN, ml);
+        tmem_wait_ld();
+        const float m_o = __uint_as_float(ml[0]), l_o = __uint_as_float(ml[1]);
+        m_row = fmaxf(m_used, m_o);
+        const float mine = weight(m_used, m_row), other = weight(m_o, m_row);
+        l_row = mine * l + other * l_o;
+        w0 = t == 0 ? mine : other, w1 = t == 0 ? other : mine;
+        // Whether a tile took a block at all: the same for all its rows.
+        any0 = j0 + (j0 & 1) < j0 + seg, any1 = j0 + 1 - (j0 & 1) < j0 + seg;
+      } else {
+        w0 = w1 = m_used == -INFINITY ? 0.f : 1.f;
+      }
+      const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);
+      const float scale = direct ? inv : 1.f;
+      w0 *= scale, w1 *= scale;
+      float* share = direct ? nullptr : slot_of(me);
+      if (quad_rows > 0) {
+        if (c0 == 0 && lane < quad_rows) {
+          if (!direct) {
+            *reinterpret_cast<float2*>(share + kWideRows * D + 2 * (t * kTileM + r)) = make_float2(m_row, l_row);
+          } else if (p.lse) {
+            const Row at = query_row(w, it, row_begin + r);
+            p.lse[((int64_t)at.b * p.n + at.i) * p.H + at.head] = l_row == 0.f ? -INFINITY : (m_row + log2f(l_row)) * kLn2;
+          }
+        }
+#pragma unroll 1
+        for (int cb = c0; cb < c1; cb += D / 2) {
+#pragma unroll 1
+          for (int x = 0; x < D / 64; ++x) {
+            uint32_t ov[32];
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            if (any0) {
+              tmem_ld32(tmem + lane_off + C::kOCol + cb + x * 32, ov);
+              tmem_wait_ld();
+              if (w0 != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = w0 * __uint_as_float(ov[i]);
+              }
+            }
+            __syncwarp();
+            if (any1) {
+              tmem_ld32(tmem + lane_off + C::kOCol + D + cb + x * 32, ov);
+              tmem_wait_ld();
+              if (w1 != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += w1 * __uint_as_float(ov[i]);
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+          __syncwarp();
+          if (!direct) {  // 4 values a lane, whole rows of D / 2 values
+            constexpr int kLanes = D / 8;
+            const int col = lane % kLanes * 4;
+            float* dst = share + (step == 2 ? 0 : t * kTileM) * D + cb + col;
+#pragma unroll 4
+            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes)
+              *reinterpret_cast<float4*>(dst + (quad * 32 + rr) * D) = *stage_at(quad * 32 + rr, col);
+          } else {  // 8 values a lane
+            constexpr int kLanes = D / 16;
+            const int col = lane % kLanes * 8;
+#pragma unroll 2
+            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes) {
+              const Row at = query_row(w, it, row_begin + quad * 32 + rr);
+              const float4 a = *stage_at(quad * 32 + rr, col), b = *stage_at(quad * 32 + rr, col + 4);
+              if (cb + col < p.D)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh + cb +
+                                          col) =
+                    make_uint4(pack2<kBf16>(a.x, a.y), pack2<kBf16>(a.z, a.w), pack2<kBf16>(b.x, b.y), pack2<kBf16>(b.z, b.w));
+            }
+          }
+          __syncwarp();
+        }
+      }
+      // O_t has been read: the next item's first PV_t may overwrite it once p_half says so.  With
+      // two halves the other tile's warps read it too, and Q_0 is shared.
+      tc_fence_before();
+      if (step == 2 || (!direct && !w.prefix_pass))
+        if (!(ok = meet())) break;
+      if (!direct && !w.prefix_pass) {
+        // The last block to leave its share of the item joins them all.
+        if (threadIdx.x == 0) {
+          __threadfence();
+          *s_last = atomicAdd(&p.counters[cf], 1) == cl - cf;
+        }
+        if (!(ok = meet())) break;
+        if (*s_last) {
+          __threadfence();
+          if (p.pre.slots) griddep_wait();  // the prefix's shares are complete
+          constexpr int kLanes = D / 4;  // 4 values a lane
+          const int col = lane % kLanes * 4;
+          // With two halves the tiles' warps share the rows of a quadrant.
+          const int first_row = step == 2 ? t * 16 : 0, end_row = min(quad_rows, step == 2 ? first_row + 16 : 32);
+#pragma unroll 1
+          for (int rr = first_row + lane / kLanes; rr < end_row; rr += 32 / kLanes) {
+            const int tile_row = (step == 2 ? 0 : t * kTileM) + quad * 32 + rr;
+            const Row at = query_row(w, it, row_begin + quad * 32 + rr);
+            float mm = -INFINITY, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            join_shares<D, 4, 4>(
+                cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kWideRows, tile_row, col, mm, ll, v);
+            if (p.pre.slots)
+              join_prefix<D, 4, 4>(p.pre, p.Hk, it.hk, (int64_t)at.b * p.rows + (int64_t)at.i * p.G + at.head - it.hk * p.G, col,
+                                   mm, ll, v);
+            const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+            if (col < p.D)
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh + col) =
+                  make_uint2(pack2<kBf16>(v[0] * inv, v[1] * inv), pack2<kBf16>(v[2] * inv, v[3] * inv));
+            if (col == 0 && p.lse)
+              p.lse[((int64_t)at.b * p.n + at.i) * p.H + at.head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+          }
+          if (threadIdx.x == 0) p.counters[cf] = 0;
+        }
+        if (!(ok = meet())) break;  // s_last is read before the next item writes it
+      }
+      // Past this item's share.
+      Item nx = it;
+      const bool more = walk->done + seg < walk->todo;
+      if (more) next_item(w, nx);
+      __syncwarp();
+      if (lane == 0) {
+        walk->it.b = nx.b, walk->it.hk = nx.hk, walk->it.pair = nx.pair;
+        walk->it.units = nx.units, walk->it.keys = nx.keys, walk->it.visible = nx.visible;
+        walk->j0 = 0, walk->item = item + 1;
+        walk->unit = walk->unit + seg;
+        walk->done = walk->done + seg;
+      }
+      __syncwarp();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <int D, bool kBf16>
+int launch(const CUtensorMap& tk, const CUtensorMap& tv, const WideParams& w, int grid, bool dependent, cudaStream_t s) {
+  auto kern = paged_wide_kernel<D, kBf16>;
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+    if (e != cudaSuccess) return cuda_status(e);
+    configured.fetch_or(bit);
+  }
+  return launch_kernel(kern, grid, kThreads, Cfg<D>::kSmem, dependent, s, tk, tv, w);
+}
+
+// Cache pages as a [page][head][row][d] tensor, boxes of 64 values x box_rows rows.
+int page_map(CUtensorMap* map, bool bf16, const void* base, const Params& p, int64_t sp, int64_t ss, int64_t sh, int box_rows) {
+  const uint64_t dims[4] = {(uint64_t)p.D, (uint64_t)p.page_size, (uint64_t)p.Hk, (uint64_t)p.num_pages};
+  const uint64_t strides[3] = {(uint64_t)ss * 2, (uint64_t)sh * 2, (uint64_t)sp * 2};
+  const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
+  return make_tmap(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+                   CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace
+
+int wide_box_rows(int page_size) {
+  int r = 1;
+  while (r < 128 && page_size % (2 * r) == 0) r *= 2;
+  return r >= 8 ? r : 0;
+}
+
+int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units, cudaStream_t s) {
+  WideParams w{};
+  w.p = p;
+  w.prefix_pass = prefix_pass;
+  w.rows = prefix_pass ? (int64_t)p.B * p.rows : p.rows;
+  w.halves = w.rows <= kTileM ? 2 : 1;
+  const int64_t tile = w.halves == 2 ? kTileM : 2 * kTileM;
+  w.pairs = (int)((w.rows + tile - 1) / tile);
+  w.box_rows = wide_box_rows(p.page_size);
+  w.lines = 1;
+  int64_t grid = sm_count();
+  if (prefix_pass) {
+    w.lines = p.pre.lines;
+    grid = (int64_t)p.pre.lines * p.pre.nc;
+  } else if (grid > max_units) {
+    grid = max_units;
+  }
+  CUtensorMap tk, tv;
+  if (int st = page_map(&tk, bf16, p.k, p, p.k_sp, p.k_ss, p.k_sh, w.box_rows)) return st;
+  if (int st = page_map(&tv, bf16, p.v, p, p.v_sp, p.v_ss, p.v_sh, w.box_rows)) return st;
+  const bool dependent = !prefix_pass && p.pre.slots != nullptr;
+  if (p.D > 64)
+    return bf16 ? launch<128, true>(tk, tv, w, (int)grid, dependent, s) : launch<128, false>(tk, tv, w, (int)grid, dependent, s);
+  return bf16 ? launch<64, true>(tk, tv, w, (int)grid, dependent, s) : launch<64, false>(tk, tv, w, (int)grid, dependent, s);
+}
+
+}  // namespace paged
+}  // namespace lk

@@ -89,7 +89,7 @@ SIGNATURES = {
         [_p, _p, _p, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _b64, _p, _i64, _i64,
          _i64, _b64, _i, _p],
     ),
-    "lk_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "lk_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "lk_paged_attention": (
         _i,
         [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p, _i64, _p],

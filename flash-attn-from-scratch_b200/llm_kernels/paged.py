@@ -116,8 +116,8 @@ def paged_kv_append(k, v, k_cache, v_cache, slots, *, q=None, positions=None, co
 _workspaces: dict = {}
 
 
-def _workspace(dev, stream, B, n, H, Hk, D):
-    need = _lib.load().lk_paged_attention_workspace_bytes(B, n, H, Hk, D)
+def _workspace(dev, stream, B, n, H, Hk, D, prefix):
+    need = _lib.load().lk_paged_attention_workspace_bytes(B, n, H, Hk, D, prefix)
     if torch.cuda.is_current_stream_capturing():
         # A graph may be replayed beside this stream's other work: it keeps a workspace of its own.
         return torch.zeros(need, dtype=torch.uint8, device=dev), need
@@ -172,7 +172,7 @@ def _attention(name, q, k_cache, v_cache, prefix, block_table, lengths, softmax_
     lse = torch.empty((B, n, H), dtype=torch.float32, device=dev) if return_lse else None
     if B and n and H:
         stream = stream_for(dev)
-        ws, ws_bytes = _workspace(dev, stream, B, n, H, Hk, D)
+        ws, ws_bytes = _workspace(dev, stream, B, n, H, Hk, D, prefix[1] if prefix else 0)
         strides = _lib.pack_i64(*qs[:3], *out.stride()[:3], *ks[:3], *vs[:3])
         head = (ptr(q), ptr(k_cache), ptr(v_cache))
         tail = (ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(lengths), ptr(out),

@@ -383,7 +383,8 @@ LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const v
  * prefix_length keys, held in the pages prefix_pages[0 ..]; every token sees all of them, and
  * they are read and multiplied once for the whole batch.  block_table and lengths name what
  * follows the prefix, from the start of a page of its own; lengths[b] may be 0. */
-LK_API int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D);
+LK_API int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D,
+                                                  int64_t prefix_length);
 LK_API int lk_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                               int64_t table_ld, int64_t table_cols, const int32_t* lengths, void* out, float* lse,
                               const int64_t* strides, int dtype, int64_t B, int64_t n, int64_t H, int64_t H_kv,
