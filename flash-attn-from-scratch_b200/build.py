@@ -3,7 +3,9 @@
 Every ``csrc/*.cu`` file is compiled for ``sm_100a`` only (relocatable device code, so the
 device status word is one symbol shared by all kernels), then device-linked and linked into
 one shared library with the CUDA runtime linked statically.  The library needs no torch and
-exports exactly the functions declared in ``include/llm_kernels_b200.h``.
+exports exactly the functions declared in ``include/llm_kernels_b200.h``.  ``csrc/binding.cpp``
+becomes ``llm_kernels/_binding.so``, a CPython extension over that library (g++; Python's headers
+and the DLPack header that torch ships, nothing linked to torch).
 
 Usage::
 
@@ -16,16 +18,19 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "llm_kernels", "liblk_b200.so")
+BINDING = os.path.join(HERE, "llm_kernels", "_binding.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -76,6 +81,19 @@ def _compile(src: str, verbose: bool) -> tuple[str, str]:
     return obj, (r.stderr if verbose else "")
 
 
+def _build_binding(force: bool) -> None:
+    src = os.path.join(CSRC, "binding.cpp")
+    if not force and not _stale(BINDING, [src, OUT, *_headers()]):
+        return
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(torch_dir, "include"), src, "-o", BINDING,
+           "-L" + os.path.dirname(OUT), "-l:" + os.path.basename(OUT), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for binding.cpp:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
@@ -95,6 +113,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         for log in logs:
             sys.stderr.write(log)
+    _build_binding(force)
     return OUT
 
 

@@ -1,15 +1,15 @@
 """ctypes binding of the C ABI in ``include/llm_kernels_b200.h`` (``liblk_b200.so``).
 
-This is the only way the Python layer reaches the GPU: every op calls one of these entry
-points with raw device pointers, element strides and torch's current CUDA stream.  There is
-no other code path — if the library is missing, the ops raise instead of computing anything.
+The Python layer reaches the GPU only through these entry points, with raw device pointers,
+element strides and torch's current CUDA stream: by ctypes, or for the serving operators, whose
+calls are small, by a CPython extension over the same library (``binding``).  There is no other
+code path — if the library is missing, the ops raise instead of computing anything.
 """
 
 from __future__ import annotations
 
 import ctypes
 import os
-import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -36,7 +36,6 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
 _pi64 = ctypes.POINTER(ctypes.c_int64)
-_b64 = ctypes.c_char_p  # const int64_t* given as packed bytes (pack_i64): no array object per call
 
 # name -> (restype, argtypes); mirrors include/llm_kernels_b200.h one for one.
 SIGNATURES = {
@@ -82,21 +81,21 @@ SIGNATURES = {
     ),
     "lk_rotary_embed": (
         _i,
-        [_p, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _b64, _p, _i64, _i64, _i64, _b64, _i, _i, _p],
+        [_p, _p, _p, _p, _pi64, _i, _i64, _i64, _i64, _i64, _i64, _p, _i, _pi64, _p, _i64, _i64, _i64, _pi64, _i, _i, _p],
     ),
     "lk_paged_kv_append": (
         _i,
-        [_p, _p, _p, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _b64, _p, _i64, _i64,
-         _i64, _b64, _i, _p],
+        [_p, _p, _p, _p, _p, _p, _pi64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _pi64, _p, _i64, _i64,
+         _i64, _pi64, _i, _p],
     ),
     "lk_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "lk_paged_attention": (
         _i,
-        [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p, _i64, _p],
+        [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _pi64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p, _i64, _p],
     ),
     "lk_shared_prefix_attention": (
         _i,
-        [_p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _b64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p,
+        [_p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _p, _pi64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p,
          _i64, _p],
     ),
     "lk_rmsnorm_linear_fold": (_i, [_p, _i, _p, _p, _i, _i64, _i64, _p]),
@@ -142,6 +141,39 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def _call_error(name: str, status: int, cuda: int) -> LKError:
+    return LKError(name, status, f"cudaError {cuda}" if cuda else "")
+
+
+def binding():
+    """The CPython extension of the serving operators (csrc/binding.cpp), set up once."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    load()
+    with _lock:
+        if _binding is None:
+            import torch
+
+            from . import _binding as ext
+            from ._common import LKInputError
+
+            ext.setup(
+                torch.Tensor,
+                torch.empty_like,
+                lambda q: torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device),
+                torch.cuda.is_current_stream_capturing,
+                lambda dev, n: torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda", dev)),
+                LKInputError,
+                _call_error,
+            )
+            _binding = ext
+    return _binding
+
+
 def status_string(status: int) -> str:
     try:
         return load().lk_status_string(int(status)).decode()
@@ -162,11 +194,6 @@ def call(name: str, *args) -> None:
 
 def i64_array(vals) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
-
-
-def pack_i64(*vals) -> bytes:
-    """int64 values as the bytes that a ``const int64_t*`` parameter points to."""
-    return struct.pack("%dq" % len(vals), *vals)
 
 
 _tls = threading.local()
@@ -192,6 +219,8 @@ def device_status() -> tuple[int, int, int, int]:
 
 def clear_device_status() -> None:
     call("lk_clear_device_status")
+    if _binding is not None:
+        _binding.drop_workspaces()  # their counters are not to be trusted after a failure
 
 
 def exported_symbols() -> list[str]:
