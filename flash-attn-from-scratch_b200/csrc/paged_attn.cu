@@ -7,19 +7,26 @@
 //
 // Bound: memory.  Each key and value is read once for at most 16 rows (4 D bytes for 64 D flops
 // per key and head at 16 rows: 16 flop/byte, and the card's balance is ~250), so the work is to
-// keep reads in flight.  Four warps of a block take 16 keys each of every 64-key unit and run
-// without any barrier between them until an item ends: a warp has its own ring of stages in
-// shared memory, filled by 16-byte cp.async -- row by row through the block table, so pages of
-// any size and caches of any stride take the same path, and rows behind the last key are filled
-// with zeros instead of read -- and its own running (m, l, O), kept in registers.  The rows of
-// a K/V head's query group fill the 16 rows of mma.sync's A operand, and S's accumulator layout
-// is P's operand layout, so P never leaves registers.  (tcgen05 would need 128 rows and a trip
+// keep reads in flight.  The warps of a block run without any barrier between them until an item
+// ends: a warp takes 16 keys a step, has its own ring of stages in shared memory, filled by
+// 16-byte cp.async -- row by row through the block table, so pages of any size and caches of any
+// stride take the same path, and rows behind the last key are filled with zeros instead of read
+// -- and its own running (m, l, O), kept in registers.  The rows of a K/V head's query group fill
+// the 16 rows of mma.sync's A operand, and S's accumulator layout is P's operand layout, so P
+// never leaves registers.  (tcgen05 would need 128 rows and a trip
 // through tensor memory for the same 16; its throughput is not what bounds this kernel.)
 // Loads run ahead across the ends of items, so short sequences do not drain the ring.
+//
+// A team is the warps that share an item: four where there are few items (their shares meet in
+// shared memory, a quarter as many go through the workspace), one where there are many (an item's
+// end then holds up one warp, not four).
 #include <atomic>
 
+#include <cstdlib>
 #include "lk_abi.h"
 #include "paged_common.cuh"
+static int64_t many_items() { const char* e = getenv("LK_MI"); return e ? atoll(e) : 256; }
+static int64_t prefix_pass() { const char* e = getenv("LK_PT"); return e ? atoll(e) : 1024; }
 
 namespace lk {
 namespace paged {
@@ -28,28 +35,20 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;              // query rows of an item
 constexpr int kGroup = 16;             // keys of one warp's step
-constexpr int kUnit = kWarps * kGroup;  // keys of a unit
-constexpr int kStages = 3;
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 // Units of 64 prefix keys, over all sequences and K/V heads, from which the prefix pass pays.
 constexpr int64_t kPrefixPass = 1024;
+// Items from which a team is one warp.
+constexpr int64_t kManyItems = 256;
 
 template <int DP>
 struct Cfg {
+  static constexpr int kStages = DP == 128 ? 3 : 6;          // of a warp's ring: 24 KB
   static constexpr int kTile = kGroup * DP * 2;              // bytes of a warp's K or V tile
   static constexpr int kRing = kWarps * kStages * 2 * kTile;
   static constexpr int kJoin = kWarps * 8 * DP * 4;          // 8 rows of every warp's O
   static constexpr int kSmem = kRing + kJoin + kWarps * kRows * 2 * 4;
 };
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int n>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -77,7 +76,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A place on the line of units.
+// A place on the line of units: a team's step is kUnit keys.
+template <int kUnit>
 struct Place {
   int b, hk, rt;  // item: sequence, K/V head, tile of 16 rows
   int j, units;   // unit of the item, and how many it has
@@ -98,68 +98,74 @@ struct Place {
   }
 };
 
-template <int DP, bool kBf16>
+template <int DP, bool kBf16, int kTeam>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params p) {
   using C = Cfg<DP>;
+  constexpr int kStages = C::kStages;
+  constexpr int kUnit = kTeam * kGroup;
+  constexpr int kTeams = kWarps / kTeam;   // of a block
   constexpr int kChunks = DP / 8;          // 16-byte pieces of a row
   constexpr int kPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
+  constexpr int kPer = DP / 32;            // columns of a lane where a warp has whole rows
+  griddep_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sO = reinterpret_cast<float*>(smem + C::kRing);                // [kWarps][8][DP], swizzled
-  float* sM = reinterpret_cast<float*>(smem + C::kRing + C::kJoin);     // [kWarps][kRows]
+  float* sO = reinterpret_cast<float*>(smem + C::kRing);              // [kWarps][8][DP], swizzled
+  float* sM = reinterpret_cast<float*>(smem + C::kRing + C::kJoin);   // [kWarps][kRows]
   float* sL = sM + kWarps * kRows;
   __shared__ int s_last;
+  __shared__ int2 s_found[kTeams];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int in_team = warp % kTeam;  // this warp's place in its team
   const int tiles = (p.rows + kRows - 1) / kRows;
   const int per_seq = p.Hk * tiles;
+  const int c = blockIdx.x * kTeams + warp / kTeam;  // this warp's team
   Line line;
-  const int c = blockIdx.x;
-  const Found found = locate<kThreads>(
-      p.B, per_seq, reinterpret_cast<long long*>(sM), &line.units,
-      [&](int b) { return max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit); },
-      [&](int64_t U) {
-        line.units = U;
-        line.nc = (int)min((int64_t)gridDim.x, U);  // every block that takes part has a unit
-        return c < line.nc ? line.begin(c) : 0;
-      });
-  Place at;
-  at.b = found.b;
-  at.enter(p);
-  at.hk = (int)(found.offset / at.units);
-  at.j = (int)(found.offset - (int64_t)at.hk * at.units);
-  at.rt = at.hk % tiles;
-  at.hk /= tiles;
+  if (!locate<kThreads, kTeams>(p.B, gridDim.x * kTeams, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
+                                [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; }))
+    return;
   if (c >= line.nc) return;
-  const int64_t u0 = line.begin(c);
-  const int todo = (int)(line.begin(c + 1) - u0);  // units of this block
+  Place<kUnit> at;
+  at.b = s_found[warp / kTeam].x;
+  at.enter(p);
+  const int offset = s_found[warp / kTeam].y;
+  at.hk = (int)((unsigned)offset / (unsigned)at.units);
+  at.j = offset - at.hk * at.units;
+  at.rt = 0;
+  if (tiles > 1) {
+    const int item = at.hk;
+    at.hk = item / tiles;
+    at.rt = item - at.hk * tiles;
+  }
+  const int u0 = line.begin(c);
+  const int todo = line.begin(c + 1) - u0;  // units of this team
 
   // ------------------------------------------------------------------ loads
   const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * C::kTile);
   const int chunk = lane % kChunks, sub = lane / kChunks;
   const bool chunk_in = chunk * 8 < p.D;
-  Place ld = at;
+  Place<kUnit> ld = at;
   int ld_left = todo;
-  // Lane l (and l + 16) looks up the page of key l of this warp's group, one step ahead.
-  auto look_up = [&]() {
-    const int t = ld.j * kUnit + warp * kGroup + (lane & 15);
+  // Lane l (and l + 16) looks up the page of key l of this warp's step, one step ahead; the entry
+  // is not looked at before its turn.
+  auto look_up = [&](int& in) {
+    const int t = ld.j * kUnit + in_team * kGroup + (lane & 15);
+    in = 0;
     if (ld_left <= 0 || t >= ld.keys) return -1;
-    const int o = t - p.prefix;
-    const int page = o < 0 ? p.prefix_pages[t / p.page_size] : p.table[ld.b * p.table_ld + o / p.page_size];
-    if ((unsigned)page >= (unsigned)p.num_pages) {
-      record_bad_index(kSitePage);
-      return -1;
-    }
-    return page;
+    const int o = t - p.prefix, x = o < 0 ? t : o;
+    const int col = p.by_page.div(x);
+    in = x - col * p.page_size;
+    return o < 0 ? p.prefix_pages[col] : p.table[ld.b * p.table_ld + col];
   };
-  int page = look_up();
+  int in_next;
+  int page = look_up(in_next);
   int ld_stage = 0;
   auto load = [&]() {
     if (ld_left > 0) {
-      const int t = ld.j * kUnit + warp * kGroup + (lane & 15);
-      const int o = t - p.prefix;
-      const int in = (o < 0 ? t : o) % p.page_size;
-      const int64_t ok = page < 0 ? -1 : page * p.k_sp + in * p.k_ss + ld.hk * p.k_sh;
-      const int64_t ov = page < 0 ? -1 : page * p.v_sp + in * p.v_ss + ld.hk * p.v_sh;
+      const bool held = (unsigned)page < (unsigned)p.num_pages;
+      if (!held && ld.j * kUnit + in_team * kGroup + (lane & 15) < ld.keys) record_bad_index(kSitePage);
+      const int64_t ok = held ? page * p.k_sp + in_next * p.k_ss + ld.hk * p.k_sh : -1;
+      const int64_t ov = held ? page * p.v_sp + in_next * p.v_ss + ld.hk * p.v_sh : -1;
       const uint32_t dst = ring + ld_stage * (2 * C::kTile);
 #pragma unroll
       for (int i = 0; i < kGroup / kPerCopy; ++i) {
@@ -172,17 +178,16 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
       }
       ld.advance(p, tiles);
       --ld_left;
-      page = look_up();
+      page = look_up(in_next);
       ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
     }
     cp_commit();
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) load();
 
   // ------------------------------------------------------------------ items
-  int stage = 0;
-  int64_t unit = u0;
+  int stage = 0, unit = u0;
   const int r0 = lane >> 2;  // this lane's rows: r0 and r0 + 8
   for (int done = 0; done < todo;) {
     const int seg = min(at.units - at.j, todo - done);  // units of this item here
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     for (int h = 0; h < 2; ++h) {
       const int row = at.rt * kRows + r0 + 8 * h;
       const bool in = row < p.rows;
-      const int i = in ? row / p.G : 0, g = in ? row - i * p.G : 0;
+      const int i = in ? p.by_G.div(row) : 0, g = in ? row - i * p.G : 0;
       // Keys below lim are seen: the prefix and the own keys up to the token's own.
       lim[h] = p.prefix + max(0, at.keys - p.prefix - p.n + i + 1);
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb + i * p.q_ss +
@@ -205,13 +210,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
         qf[ks][2 + h] = in && d + 8 < p.D ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
       }
     }
-    // Tokens see at least this many keys: units below need no mask.
+    // Tokens see at least this many keys: steps below need no mask.
     const int all_see = p.prefix + max(0, at.keys - p.prefix - p.n + 1);
     float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
+#pragma unroll 1
     for (int s = 0; s < seg; ++s) {
       cp_wait<kStages - 2>();
       __syncwarp();
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
           mma16816<kBf16>(x[1], qf[ks], kf[2], kf[3]);
         }
       }
-      const int t0 = (at.j + s) * kUnit + warp * kGroup;
+      const int t0 = (at.j + s) * kUnit + in_team * kGroup;
       if (t0 + kGroup > all_see) {
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
@@ -285,7 +291,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     }
 
     // ---------------------------------------------------------------- end of the item's share
-    const int64_t item0 = unit - at.j;  // the item's first unit
+    auto team_sync = [&]() {
+      if constexpr (kTeam == 1) __syncwarp();
+      else __syncthreads();
+    };
+    const int item0 = unit - at.j;  // the item's first unit
     const int cf = line.block_of(item0), cl = line.block_of(item0 + at.units - 1);
     const bool split = cf != cl;
 #pragma unroll
@@ -299,50 +309,45 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
       }
     }
     const int rows_here = min(kRows, p.rows - at.rt * kRows);
-    // Slot of block x's share of a split item: 2 x if it began before x, else 2 x + 1.
+    // Slot of team x's share of a split item: 2 x if it began before x, else 2 x + 1.
     auto slot_of = [&](int x) { return p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kRows * (DP + 2); };
-    constexpr int kPer = 8 * DP / kThreads;  // values of 8 rows that a thread joins (8 or 4)
-    const int jr = threadIdx.x / (DP / kPer), jd = threadIdx.x % (DP / kPer) * kPer;
+    const int col = lane * kPer;  // from here on a warp has whole rows
     auto write_out = [&](int row, float mm, float ll, float (&v)[kPer]) {
       const int q_row = at.rt * kRows + row;
-      const int i = q_row / p.G, g = q_row - i * p.G, head = at.hk * p.G + g;
-      if (p.pre.slots) join_prefix<DP, kPer, 8>(p.pre, p.Hk, at.hk, (int64_t)at.b * p.rows + q_row, jd, mm, ll, v);
+      const int i = p.by_G.div(q_row), g = q_row - i * p.G, head = at.hk * p.G + g;
+      if (p.row_share) return leave_row<DP, kPer>(p, (at.b * p.n + i) * p.H + head, col, mm, ll, v);
       const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-      if (jd < p.D) {
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + at.b * p.o_sb + i * p.o_ss + head * p.o_sh + jd;
-        uint32_t w[kPer / 2];
-#pragma unroll
-        for (int e = 0; e < kPer / 2; ++e) w[e] = pack2<kBf16>(v[2 * e] * inv, v[2 * e + 1] * inv);
-        if constexpr (kPer == 8)
-          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (col < p.D) {
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + at.b * p.o_sb + i * p.o_ss + head * p.o_sh + col;
+        if constexpr (kPer == 4)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(v[0] * inv, v[1] * inv), pack2<kBf16>(v[2] * inv, v[3] * inv));
         else
-          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint32_t*>(dst) = pack2<kBf16>(v[0] * inv, v[1] * inv);
       }
-      if (p.lse && jd == 0)
+      if (p.lse && col == 0)
         p.lse[((int64_t)at.b * p.n + i) * p.H + head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
     };
-#pragma unroll
-    if (p.pre.slots) griddep_wait();  // the prefix's shares are complete
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half * 8 >= rows_here) break;
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i) {
         const int d = i * 8 + 2 * (lane & 3);
-        *reinterpret_cast<float2*>(sO + (warp * 8 + r0) * DP + (d ^ ((r0 & 7) * 8 % DP))) =
+        *reinterpret_cast<float2*>(sO + (warp * 8 + r0) * DP + (d ^ (r0 * 8 % DP))) =
             make_float2(o[i][half ? 2 : 0], o[i][half ? 3 : 1]);
       }
-      __syncthreads();
-      const int row = half * 8 + jr;
-      if (row < rows_here) {
-        float mw[kWarps], mm = -INFINITY, ll = 0.f, v[kPer] = {};
+      team_sync();
+#pragma unroll 1
+      for (int jr = in_team; jr < min(8, rows_here - half * 8); jr += kTeam) {
+        const int row = half * 8 + jr, first = warp - in_team;
+        float mw[kTeam], mm = -INFINITY, ll = 0.f, v[kPer] = {};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mw[w] = sM[w * kRows + row], mm = fmaxf(mm, mw[w]);
+        for (int w = 0; w < kTeam; ++w) mw[w] = sM[(first + w) * kRows + row], mm = fmaxf(mm, mw[w]);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kTeam; ++w) {
           const float a = weight(mw[w], mm);
-          ll += a * sL[w * kRows + row];
-          const float* src = sO + (w * 8 + jr) * DP + (jd ^ (jr * 8 % DP));
+          ll += a * sL[(first + w) * kRows + row];
+          const float* src = sO + ((first + w) * 8 + jr) * DP + (col ^ (jr * 8 % DP));
 #pragma unroll
           for (int e = 0; e < kPer; ++e) v[e] += a * src[e];
         }
@@ -350,30 +355,37 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
           write_out(row, mm, ll, v);
         } else {
           float* dst = slot_of(c);
-          if (jd == 0) *reinterpret_cast<float2*>(dst + kRows * DP + 2 * row) = make_float2(mm, ll);
-#pragma unroll
-          for (int e = 0; e < kPer; e += 4)
-            *reinterpret_cast<float4*>(dst + row * DP + jd + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          if (col == 0) *reinterpret_cast<float2*>(dst + kRows * DP + 2 * row) = make_float2(mm, ll);
+          if constexpr (kPer == 4)
+            *reinterpret_cast<float4*>(dst + row * DP + col) = make_float4(v[0], v[1], v[2], v[3]);
+          else
+            *reinterpret_cast<float2*>(dst + row * DP + col) = make_float2(v[0], v[1]);
         }
       }
-      __syncthreads();
+      team_sync();
     }
     if (split) {
-      if (threadIdx.x == 0) {
+      int last = 0;
+      if (lane == 0 && in_team == 0) {
         __threadfence();
-        s_last = atomicAdd(&p.counters[cf], 1) == cl - cf;
+        last = atomicAdd(&p.counters[cf], 1) == cl - cf;
+        if (kTeam > 1) s_last = last;
       }
-      __syncthreads();
-      if (s_last) {
+      if constexpr (kTeam > 1) {
+        __syncthreads();
+        last = s_last;
+      } else {
+        last = __shfl_sync(~0u, last, 0);
+      }
+      if (last) {
         __threadfence();
-        for (int half = 0; half < (rows_here + 7) / 8; ++half) {
-          const int row = half * 8 + jr;
-          if (row >= rows_here) continue;
+#pragma unroll 1
+        for (int row = in_team; row < rows_here; row += kTeam) {
           float mm = -INFINITY, ll = 0.f, v[kPer] = {};
-          join_shares<DP, kPer, 8>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, row, jd, mm, ll, v);
+          join_shares<DP, kPer, 8>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, row, col, mm, ll, v);
           write_out(row, mm, ll, v);
         }
-        if (threadIdx.x == 0) p.counters[cf] = 0;
+        if (lane == 0 && in_team == 0) p.counters[cf] = 0;
       }
     }
     // Past this item.
@@ -383,12 +395,48 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     at.advance(p, tiles);
   }
   cp_wait<0>();
+  // The join of the prefix's shares waits for this kernel, and so for the prefix pass before it.
+  if (p.row_share) griddep_wait();
+}
+
+// One warp for each query row: its sums over its own keys and the prefix's shares of it, to `out`.
+// Bound: latency of the loads, all of a batch in flight at once; a pass of its own, because a block
+// of the kernels over the sequences' own keys would wait for it at the end of every sequence.
+template <int DP, bool kBf16>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const Params p) {
+  constexpr int kPer = DP / 32;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  griddep_wait();
+  if (row >= p.B * p.n * p.H) return;
+  const int token = row / p.H, head = row - token * p.H, b = token / p.n, i = token - b * p.n;
+  const int hk = p.by_G.div(head), col = lane * kPer;
+  using V = typename std::conditional<kPer % 4 == 0, float4, float2>::type;
+  float v[kPer];
+  *reinterpret_cast<V*>(v) = __ldcg(reinterpret_cast<const V*>(p.row_share + (int64_t)row * DP + col));
+  const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row));
+  float mm = ml.x, ll = ml.y;
+  join_prefix<DP, kPer, 8>(p.pre, p.Hk, hk, b * p.rows + i * p.G + head - hk * p.G, col, mm, ll, v);
+  const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+  if (col < p.D) {
+    uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o_sb + i * p.o_ss + head * p.o_sh + col;
+    if constexpr (kPer == 4)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(v[0] * inv, v[1] * inv), pack2<kBf16>(v[2] * inv, v[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(dst) = pack2<kBf16>(v[0] * inv, v[1] * inv);
+  }
+  if (p.lse && col == 0) p.lse[row] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
 }
 
 template <int DP, bool kBf16>
-int launch_rows16(const Params& p, int64_t max_units, cudaStream_t s) {
+int launch_join(const Params& p, cudaStream_t s) {
+  const int rows = p.B * p.n * p.H;
+  return launch_kernel(paged_join_kernel<DP, kBf16>, (rows + kWarps - 1) / kWarps, kThreads, 0, true, s, p);
+}
+
+template <int DP, bool kBf16, int kTeam>
+int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
   using C = Cfg<DP>;
-  auto kern = paged_rows16_kernel<DP, kBf16>;
+  auto kern = paged_rows16_kernel<DP, kBf16, kTeam>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -399,9 +447,17 @@ int launch_rows16(const Params& p, int64_t max_units, cudaStream_t s) {
     configured.fetch_or(bit);
   }
   int64_t grid = 2 * (int64_t)sm_count();
-  if (grid > max_units) grid = max_units;
-  if (grid > kCounters) grid = kCounters;
-  return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.pre.slots != nullptr, s, p);
+  constexpr int64_t kUnit = kTeam * kGroup, kTeams = kWarps / kTeam;
+  const int64_t most = items * (keys > kUnit ? (keys + kUnit - 1) / kUnit : 1);
+  if (grid * kTeams > most) grid = (most + kTeams - 1) / kTeams;
+  if (grid * kTeams > kCounters) grid = kCounters / kTeams;
+  return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.row_share != nullptr, s, p);
+}
+
+template <int DP, bool kBf16>
+int launch_rows16(const Params& p, int64_t keys, cudaStream_t s) {
+  const int64_t items = (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows);
+  return items >= many_items() ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
 }
 
 }  // namespace paged
@@ -430,7 +486,9 @@ int64_t prefix_floats(const PrefixShares& s, int64_t H_kv, int64_t DP) {
 }
 // Floats of the shares of sequences' own keys.
 int64_t own_floats(int64_t rows, int64_t DP) {
-  return rows > kRows ? (int64_t)2 * sm_count() * kWideRows * (DP + 2) : (int64_t)4 * sm_count() * kRows * (DP + 2);
+  const int64_t wide = rows > kRows ? (int64_t)2 * sm_count() * kWideRows * (DP + 2) : 0;
+  const int64_t narrow = (int64_t)4 * kWarps * sm_count() * kRows * (DP + 2);
+  return wide > narrow ? wide : narrow;
 }
 }  // namespace
 }  // namespace paged
@@ -442,7 +500,8 @@ extern "C" int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int6
   if (B < 1 || n < 1 || H < 1 || H_kv < 1 || D < 1 || prefix_length < 0) return 0;
   const int64_t DP = D > 64 ? 128 : 64, rows = n * (H / H_kv);
   int64_t floats = kCounters + own_floats(rows, DP);
-  if (prefix_length > 0) floats += prefix_floats(prefix_shares(B * rows, H_kv, prefix_length), H_kv, DP);
+  if (prefix_length > 0)
+    floats += prefix_floats(prefix_shares(B * rows, H_kv, prefix_length), H_kv, DP) + B * n * H * (DP + 2);
   return (floats * 4 + 255) / 256 * 256;
 }
 
@@ -485,6 +544,7 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   p.table_ld = table_ld, p.table_cols = (int)table_cols;
   p.B = (int)B, p.n = (int)n, p.H = (int)H, p.Hk = (int)H_kv, p.G = (int)(H / H_kv), p.D = (int)D;
   p.rows = p.n * p.G;
+  p.by_G = paged::FastDiv::of(p.G), p.by_rows = paged::FastDiv::of(p.rows), p.by_page = paged::FastDiv::of(page_size);
   p.num_pages = (int)num_pages, p.page_size = (int)page_size, p.prefix = (int)prefix_length;
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -494,20 +554,26 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   const int64_t DP = D > 64 ? 128 : 64;
   bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
   for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
-  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
+  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > prefix_pass()) {
     paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
+    if ((int64_t)pre.units * H_kv * pre.pairs > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
     pre.slots = p.partial + paged::own_floats(p.rows, DP);
     p.pre = pre;
+    p.row_share = pre.slots + paged::prefix_floats(pre, H_kv, DP);
     if (int st = paged::launch_wide(p, bf16, true, 0, s)) return st;
     p.prefix = 0;
   }
-  const int64_t keys = p.prefix + table_cols * page_size;  // at most
-  auto at_most = [&](int64_t items, int64_t unit) { return items * (keys > unit ? (keys + unit - 1) / unit : 1); };
+  const int64_t keys = p.prefix + table_cols * page_size;  // of a sequence, at most
+  int st;
   if (p.rows > paged::kRows && wide && p.prefix == 0)
-    return paged::launch_wide(p, bf16, false, at_most(B * H_kv * ((p.rows + 127) / 128), 128), s);
-  const int64_t units = at_most(B * H_kv * ((p.rows + paged::kRows - 1) / paged::kRows), paged::kUnit);
-  if (D > 64) return bf16 ? paged::launch_rows16<128, true>(p, units, s) : paged::launch_rows16<128, false>(p, units, s);
-  return bf16 ? paged::launch_rows16<64, true>(p, units, s) : paged::launch_rows16<64, false>(p, units, s);
+    st = paged::launch_wide(p, bf16, false, B * H_kv * ((p.rows + 127) / 128) * (keys > 128 ? (keys + 127) / 128 : 1), s);
+  else if (D > 64)
+    st = bf16 ? paged::launch_rows16<128, true>(p, keys, s) : paged::launch_rows16<128, false>(p, keys, s);
+  else
+    st = bf16 ? paged::launch_rows16<64, true>(p, keys, s) : paged::launch_rows16<64, false>(p, keys, s);
+  if (st != LK_OK || !p.row_share) return st;
+  if (D > 64) return bf16 ? paged::launch_join<128, true>(p, s) : paged::launch_join<128, false>(p, s);
+  return bf16 ? paged::launch_join<64, true>(p, s) : paged::launch_join<64, false>(p, s);
 }
 
 extern "C" int lk_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,

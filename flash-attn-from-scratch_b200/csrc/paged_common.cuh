@@ -13,6 +13,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "fa_common.cuh"
@@ -25,6 +26,35 @@ namespace paged {
 enum Site : int {
   kSitePage = 311,    // a page id outside the cache
   kSiteLength = 312,  // a length past the block table's room
+};
+
+// 16 bytes global -> shared memory, or 16 zeros.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and mul = ceil(2^(31 + s) / d),
+// mul d - 2^(31 + s) < d <= 2^s, so n mul / 2^(31 + s) exceeds n / d by less than 1 / d.  A 64-bit
+// division in its place is a hundred instructions, which a block that lives for microseconds
+// fetches cold.
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+  static FastDiv of(int64_t d) {
+    FastDiv f{};
+    f.d = (uint32_t)d;
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    f.mul = (uint32_t)(((1ull << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+    f.shift = 31 + s;
+    return f;
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
 constexpr int kCounters = 4096;  // ints at the workspace's start: one per block, zero between calls
@@ -57,11 +87,15 @@ struct Params {
   int B, n, H, Hk, G, D;
   int rows;                                          // query rows of a (sequence, K/V head): n G
   int num_pages, page_size, table_cols;
+  FastDiv by_G, by_rows, by_page;                    // of G, rows and page_size
   int prefix;                                        // keys before the sequences' own, common to all
   float scale_log2;
   int* counters;   // [kCounters]
   float* partial;  // slots of partial sums
   PrefixShares pre;
+  // With a prefix pass: where each query row's sums over its own keys go, O [B n H][DP] and then
+  // (m, l) of each row, for the join with the prefix's shares; nullptr: `out` is final.
+  float* row_share;
 };
 
 // Keys of sequence b in its own pages.
@@ -83,42 +117,52 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // exp2 of a difference of two log2-scaled maxima, 0 where the first is -inf (also beside -inf).
 __device__ __forceinline__ float weight(float m, float top) { return m == -INFINITY ? 0.f : fa::ex2(m - top); }
 
-// The line of units of a launch: its length, and where a block's share of it lies.
+// The line of units of a launch and its even cut: the first `more` blocks have q + 1 units, the
+// others q.
 struct Line {
-  int64_t units;  // U
-  int nc;         // blocks
-  __device__ __forceinline__ int64_t begin(int c) const { return (int64_t)c * units / nc; }
-  // The block that has unit u: the largest c with c U / nc < u + 1.
-  __device__ __forceinline__ int block_of(int64_t u) const { return (int)(((u + 1) * nc - 1) / units); }
+  int q, more, nc;
+  __device__ __forceinline__ void cut(int units, int blocks) {
+    nc = min(blocks, units);  // every block that takes part has a unit
+    q = (int)((unsigned)units / (unsigned)nc);
+    more = units - q * nc;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * q + min(c, more); }
+  __device__ __forceinline__ int block_of(int u) const {
+    const int longer = more * (q + 1);
+    return u < longer ? (int)((unsigned)u / (unsigned)(q + 1)) : more + (int)((unsigned)(u - longer) / (unsigned)q);
+  }
 };
 
-// Finds the sequence whose units hold unit u of the line, by the whole block (kThreads of it):
-// units_of(b) is a sequence's count per K/V head and per_seq the count of K/V heads.  Two passes
-// over the lengths: their sum, which `first` turns into u, and a scan up to u.  Returns the
-// sequence and u's offset among its units.  scratch: 8-byte aligned, kThreads / 32 + 2 values.
-struct Found {
-  int b;
-  int64_t offset;
-};
-template <int kThreads, class UnitsOf, class First>
-__device__ __forceinline__ Found locate(int B, int per_seq, long long* scratch, int64_t* total, UnitsOf units_of, First first) {
+// Finds where a block's teams (kTeams of them, consecutive on the line from team `team0`) begin, by
+// the whole block: units_of(b) is sequence b's count of units in 64 bits.  Two passes over the lengths: their
+// sum, by which the line is cut into `teams`, and a scan up to the places looked for.  found[i] =
+// (sequence, unit among the sequence's) for team i.  Returns false (reported) if the line does not
+// fit 31 bits, which takes 2^37 keys.  scratch: 8-byte aligned, kThreads / 32 values.
+template <int kThreads, int kTeams, class UnitsOf>
+__device__ __forceinline__ bool locate(int B, int teams, int team0, long long* scratch, int2* found, Line& line,
+                                       UnitsOf units_of) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int head = (int)threadIdx.x < B ? units_of((int)threadIdx.x) : 0;
+  const long long head = (int)threadIdx.x < B ? units_of((int)threadIdx.x) : 0;
   long long mine = head;
   for (int b = threadIdx.x + kThreads; b < B; b += kThreads) mine += units_of(b);
+#pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
   if (lane == 0) scratch[warp] = mine;
   __syncthreads();
   long long all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) all += scratch[w];
-  *total = all * per_seq;
-  const int64_t u = first(*total);
-  long long base = 0;
-  for (int b0 = 0; b0 < B; b0 += kThreads) {
+  if (all > 0x7FFFFFFF) {
+    record_bad_index(kSiteLength);
+    return false;
+  }
+  line.cut((int)all, teams);
+  const int last = line.begin(min(team0 + kTeams, line.nc) - 1);  // the last place looked for
+  int base = 0;
+  for (int b0 = 0; b0 < B && base <= last; b0 += kThreads) {
     const int b = b0 + (int)threadIdx.x;
-    const int n = b0 == 0 ? head : (b < B ? units_of(b) : 0);
+    const int n = (int)(b0 == 0 ? head : (b < B ? units_of(b) : 0));
     int scan = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -128,24 +172,24 @@ __device__ __forceinline__ Found locate(int B, int per_seq, long long* scratch, 
     __syncthreads();
     if (lane == 31) scratch[warp] = scan;
     __syncthreads();
-    long long before = base, step = 0;
+    int before = base, step = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += scratch[w];
-      step += scratch[w];
+      const int x = (int)scratch[w];
+      if (w < warp) before += x;
+      step += x;
     }
-    const long long lo = (before + scan - n) * per_seq, hi = (before + scan) * per_seq;
-    if (n > 0 && lo <= u && u < hi) {
-      scratch[kWarps] = b;
-      scratch[kWarps + 1] = u - lo;
+    const int lo = before + scan - n;
+#pragma unroll
+    for (int i = 0; i < kTeams; ++i) {
+      if (team0 + i >= line.nc) break;
+      const int u = line.begin(team0 + i) - lo;
+      if (u >= 0 && u < n) found[i] = make_int2(b, u);
     }
     base += step;
-    if (base * per_seq > u) break;
   }
   __syncthreads();
-  const Found f{(int)scratch[kWarps], (int64_t)scratch[kWarps + 1]};
-  __syncthreads();
-  return f;
+  return true;
 }
 
 template <int DP>
@@ -159,15 +203,18 @@ __device__ __forceinline__ float* prefix_slot(const PrefixShares& s, int Hk, int
 // sums (mm, ll, v), kBatch loads at a time: a share after the other, the load latencies would add up.
 template <int DP, int kPer, int kBatch, class Slot>
 __device__ __forceinline__ void join_shares(int n, Slot slot, int rows, int r, int d, float& mm, float& ll, float (&v)[kPer]) {
+  using V = typename std::conditional<kPer % 4 == 0, float4, float2>::type;
+  constexpr int kW = sizeof(V) / 4;
+#pragma unroll 1
   for (int x0 = 0; x0 < n; x0 += kBatch) {
     float2 ml[kBatch];
-    float4 f[kBatch][kPer / 4];
+    V f[kBatch][kPer / kW];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const float* s = slot(min(x0 + i, n - 1));
-      ml[i] = __ldcg(reinterpret_cast<const float2*>(s + (int64_t)rows * DP + 2 * r));
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(s + rows * DP + 2 * r));
 #pragma unroll
-      for (int e = 0; e < kPer / 4; ++e) f[i][e] = __ldcg(reinterpret_cast<const float4*>(s + (int64_t)r * DP + d + 4 * e));
+      for (int e = 0; e < kPer / kW; ++e) f[i][e] = __ldcg(reinterpret_cast<const V*>(s + r * DP + d + kW * e));
       if (x0 + i >= n) ml[i].x = -INFINITY;
     }
     float top = mm;
@@ -184,24 +231,31 @@ __device__ __forceinline__ void join_shares(int n, Slot slot, int rows, int r, i
       const float b = weight(ml[i].x, top);
       ll += b * ml[i].y;
 #pragma unroll
-      for (int e = 0; e < kPer / 4; ++e) {
-        v[4 * e] += b * f[i][e].x, v[4 * e + 1] += b * f[i][e].y;
-        v[4 * e + 2] += b * f[i][e].z, v[4 * e + 3] += b * f[i][e].w;
-      }
+      for (int e = 0; e < kPer; ++e) v[e] += b * reinterpret_cast<const float*>(&f[i][e / kW])[e % kW];
     }
   }
 }
 
+// Leaves the sums of columns d .. d + kPer of query row `row` (of B n H) for the join with the prefix.
+template <int DP, int kPer>
+__device__ __forceinline__ void leave_row(const Params& p, int row, int d, float mm, float ll, const float (&v)[kPer]) {
+  using V = typename std::conditional<kPer % 4 == 0, float4, float2>::type;
+  constexpr int kW = sizeof(V) / 4;
+  float* dst = p.row_share + (int64_t)row * DP + d;
+#pragma unroll
+  for (int e = 0; e < kPer; e += kW) *reinterpret_cast<V*>(dst + e) = *reinterpret_cast<const V*>(&v[e]);
+  if (d == 0) *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row) = make_float2(mm, ll);
+}
+
 // Adds the prefix's shares for query row `row` (of all the batch's rows of K/V head hk).
 template <int DP, int kPer, int kBatch>
-__device__ __forceinline__ void join_prefix(const PrefixShares& s, int Hk, int hk, int64_t row, int d, float& mm, float& ll,
+__device__ __forceinline__ void join_prefix(const PrefixShares& s, int Hk, int hk, int row, int d, float& mm, float& ll,
                                             float (&v)[kPer]) {
-  const int pair = (int)(row / s.tile), r = (int)(row - (int64_t)pair * s.tile);
+  const int pair = s.tile == kWideRows ? row / kWideRows : row / (kWideRows / 2), r = row - pair * s.tile;
   const int line = s.lines > 1 ? pair : 0, item = s.lines > 1 ? hk : hk * s.pairs + pair;
   Line l;
-  l.units = (int64_t)s.units * (s.lines > 1 ? Hk : Hk * s.pairs);
-  l.nc = s.nc;
-  const int cf = l.block_of((int64_t)item * s.units), cl = l.block_of((int64_t)(item + 1) * s.units - 1);
+  l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), s.nc);
+  const int cf = l.block_of(item * s.units), cl = l.block_of((item + 1) * s.units - 1);
   join_shares<DP, kPer, kBatch>(
       cl - cf + 1, [&](int x) { return prefix_slot<DP>(s, Hk, line, item, cf + x); }, kWideRows, r, d, mm, ll, v);
 }
@@ -224,7 +278,7 @@ inline int launch_kernel(void (*kern)(P...), int grid, int threads, size_t smem,
 }
 
 // The 256-row kernel (paged_wide.cu).  prefix_pass: over the prefix's keys for all the batch's
-// rows, leaving shares; otherwise over each sequence's own keys, joining the shares in p.pre.
+// rows, leaving shares; otherwise over each sequence's own keys.
 int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units, cudaStream_t s);
 // Rows of a page that one TMA box may hold (0: the 256-row kernel cannot read such pages).
 int wide_box_rows(int page_size);

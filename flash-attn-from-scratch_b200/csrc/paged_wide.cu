@@ -67,7 +67,7 @@ struct Cfg {
 struct WideParams {
   Params p;
   int prefix_pass;
-  int64_t rows;    // query rows of an item's (sequence, K/V head); prefix pass: of the K/V head
+  int rows;        // query rows of an item's (sequence, K/V head); prefix pass: of the K/V head
   int pairs;       // tiles of 256 (halves == 2: 128) rows
   int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
   int box_rows;    // rows of a page in one TMA box
@@ -86,16 +86,14 @@ struct Item {
 // needs its registers for a row of S.
 struct Walk {
   Item it;
-  int j0, done, todo, c, line_id, item, nc;
-  int64_t unit, units;
+  int j0, done, todo, c, line_id, item, unit;
+  Line line;
 };
 
 __device__ __forceinline__ int visible_keys(const WideParams& w, int L, int pair) {
   if (w.prefix_pass) return L;
-  const int64_t tile = w.halves == 2 ? kTileM : 2 * kTileM;
-  const int64_t last_row = min(w.rows, (pair + 1) * tile) - 1;
-  const int i = (int)(last_row / w.p.G);
-  return max(0, L - w.p.n + i + 1);
+  const int last_row = min(w.rows, w.halves == 2 ? kTileM : (pair + 1) * 2 * kTileM) - 1;
+  return max(0, L - w.p.n + w.p.by_G.div(last_row) + 1);
 }
 __device__ __forceinline__ int units_of_keys(int keys) { return max(1, (keys + kBlockN - 1) / kBlockN); }
 
@@ -129,17 +127,15 @@ __device__ __forceinline__ void next_item(const WideParams& w, Item& it) {
 struct Row {
   int b, i, head;
 };
-__device__ __forceinline__ Row query_row(const WideParams& w, const Item& it, int64_t row) {
+__device__ __forceinline__ Row query_row(const WideParams& w, const Item& it, int row) {
   Row r;
+  r.b = it.b;
   if (w.prefix_pass) {
-    const int per = w.p.rows;  // rows of a sequence
-    r.b = (int)(row / per);
-    row -= (int64_t)r.b * per;
-  } else {
-    r.b = it.b;
+    r.b = w.p.by_rows.div(row);
+    row -= r.b * w.p.rows;
   }
-  r.i = (int)(row / w.p.G);
-  r.head = it.hk * w.p.G + (int)(row - (int64_t)r.i * w.p.G);
+  r.i = w.p.by_G.div(row);
+  r.head = it.hk * w.p.G + row - r.i * w.p.G;
   return r;
 }
 
@@ -194,45 +190,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   Line line;
   Item first;
   int c, line_id = 0;
-  int64_t u0;
   int j_first;
   if (w.prefix_pass) {
-    line_id = w.lines > 1 ? (int)blockIdx.x % w.lines : 0;
-    c = w.lines > 1 ? (int)blockIdx.x / w.lines : (int)blockIdx.x;
-    line.nc = gridDim.x / w.lines;
+    c = blockIdx.x;
+    if (w.lines > 1) {
+      c = (int)((unsigned)blockIdx.x / (unsigned)w.lines);
+      line_id = blockIdx.x - c * w.lines;
+    }
     first.keys = p.prefix;
     first.visible = p.prefix;
-    first.units = units_of_keys(p.prefix);
-    line.units = (int64_t)first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs);
-    u0 = line.begin(c);
-    const int item = (int)(u0 / first.units);
-    j_first = (int)(u0 - (int64_t)item * first.units);
+    first.units = p.pre.units;
+    line.cut(first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs), p.pre.nc);
+    const int u = line.begin(c), item = (int)((unsigned)u / (unsigned)first.units);
+    j_first = u - item * first.units;
     first.b = 0;
-    first.hk = w.lines > 1 ? item : item / w.pairs;
-    first.pair = w.lines > 1 ? line_id : item % w.pairs;
+    first.hk = item;
+    first.pair = line_id;
+    if (w.lines == 1 && w.pairs > 1) {
+      first.hk = item / w.pairs;
+      first.pair = item - first.hk * w.pairs;
+    }
   } else {
     c = blockIdx.x;
-    const Found found = locate<kThreads>(
-        p.B, p.Hk, scratch, &line.units,
-        [&](int b) {
-          const int L = own_length(p, b);
-          int sum = 0;
-          for (int x = 0; x < w.pairs; ++x) sum += units_of_keys(visible_keys(w, L, x));
-          return sum;
-        },
-        [&](int64_t U) {
-          line.units = U;
-          line.nc = (int)min((int64_t)gridDim.x, U);
-          return c < line.nc ? line.begin(c) : 0;
-        });
+    int2* found = reinterpret_cast<int2*>(scratch + kThreads / 32);
+    // Units of one K/V head of a sequence.
+    auto per_head = [&](int L) {
+      int sum = 0;
+#pragma unroll 1
+      for (int x = 0; x < w.pairs; ++x) sum += units_of_keys(visible_keys(w, L, x));
+      return sum;
+    };
+    if (!locate<kThreads, 1>(p.B, gridDim.x, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; }))
+      return;
     if (c >= line.nc) return;
-    u0 = line.begin(c);
-    first.b = found.b;
+    first.b = found->x;
     first.keys = own_length(p, first.b);
-    int per_head = 0;
-    for (int x = 0; x < w.pairs; ++x) per_head += units_of_keys(visible_keys(w, first.keys, x));
-    first.hk = (int)(found.offset / per_head);
-    j_first = (int)(found.offset - (int64_t)first.hk * per_head);
+    const int each = per_head(first.keys);
+    first.hk = (int)((unsigned)found->y / (unsigned)each);
+    j_first = found->y - first.hk * each;
     first.pair = 0;
     enter(w, first);
     while (j_first >= first.units) {
@@ -240,8 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++first.pair;
       enter(w, first);
     }
+    __syncthreads();  // the scratch is Q's
   }
-  const int todo = (int)(line.begin(c + 1) - u0);
+  const int u0 = line.begin(c);
+  const int todo = line.begin(c + 1) - u0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -276,15 +273,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Key blocks of the item's share [j0, j1) that tile t takes: from `from` to `to` in steps of
   // `halves` (none where from >= to).
   const int step = w.halves;
-  auto tile_rows_begin = [&](const Item& it, int t) {
-    return step == 2 ? (int64_t)it.pair * kTileM : ((int64_t)it.pair * 2 + t) * kTileM;  // first row of tile t
+  auto tile_rows_begin = [&](const Item& it, int t) {  // first row of tile t
+    return step == 2 ? it.pair * kTileM : (it.pair * 2 + t) * kTileM;
   };
   auto tile_units = [&](const Item& it, int t) {  // key blocks that tile t's last row sees, at least one
-    const int64_t begin = tile_rows_begin(it, t);
+    const int begin = tile_rows_begin(it, t);
     if (begin >= w.rows) return 0;
     if (w.prefix_pass) return it.units;
-    const int i = (int)((min(w.rows, begin + kTileM) - 1) / p.G);
-    return units_of_keys(max(0, it.keys - p.n + i + 1));
+    return units_of_keys(max(0, it.keys - p.n + p.by_G.div(min(w.rows, begin + kTileM) - 1) + 1));
   };
   auto tile_range = [&](const Item& it, int t, int j0, int j1, int& from, int& to) {
     from = step == 2 ? j0 + ((j0 ^ t) & 1) : j0;
@@ -293,93 +289,110 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 8) {
     // ---------------------------------------------------------------- TMA producer
+    // Ring items in the order that the MMAs take them.  One tile after the other on a block:
+    // K_0 V_0 K_1 V_1 ...; with two halves S of the next block goes before PV of this one:
+    // K_0 K_1 V_0 K_2 V_1 ... K_last V_last-1 V_last (any other order leaves a load waiting for
+    // a slot that is freed only when it is needed).
     bool ok = true;
     int issued = 0, fixes = 0;
+    const int box = w.box_rows, boxes = kBlockN / box;
     Item it = first;
     int j = j_first;
-    const int box = w.box_rows, boxes = kBlockN / box;
     // Lane g has box g of a block: its page (-1: behind the last key) and the row in it.  Looked
     // up a block ahead, and not looked at before its turn: the load takes longer than an issue.
     auto look_up = [&](int& in) {
       const int t = j * kBlockN + lane * box;
       in = 0;
       if (lane >= boxes || t >= it.keys) return -1;
-      const int col = t / p.page_size;
+      const int col = p.by_page.div(t);
       in = t - col * p.page_size;
       return w.prefix_pass ? p.prefix_pages[col] : p.table[it.b * p.table_ld + col];
     };
-    int in_next, page_next = look_up(in_next);
-    for (int done = 0; done < todo && ok; ++done) {
-      const int in = in_next, hk = it.hk, t = j * kBlockN + lane * box;
-      int page = page_next;
-      const bool held = lane < boxes && t < it.keys;
-      // Keys of the block that the sequence has; the box that holds its end is partly not its.
-      const int have = it.keys - j * kBlockN;
-      const bool ragged = have < kBlockN && have > 0 && have % box != 0;
-      if (++j == it.units && done + 1 < todo) {
-        next_item(w, it);
-        j = 0;
+    // K or V of a block: `page` and `in` are this lane's box, `have` the keys that it holds.
+    auto copy = [&](bool is_v, int page, int in, int hk, int have) {
+      const int slot = issued % S;
+      if (!mbar_wait_warp(&kv_empty[slot], ((issued / S) & 1) ^ 1u, kSiteEmpty)) return false;
+      // The box that holds the sequence's end is partly not its: V gets zeros there.
+      const bool mend = is_v && have < kBlockN && have > 0 && have % box != 0;
+      uint64_t* bar = mend ? fix : &kv_full[slot];
+      uint8_t* dst = sRing + slot * C::kTile;
+      if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+      __syncwarp();
+      if (lane < boxes) {
+        const CUtensorMap* tm = is_v ? &tmV : &tmK;
+#pragma unroll
+        for (int x = 0; x < C::kBoxes; ++x)
+          tma_load_4d(dst + x * (kTileM * 128) + lane * box * 128, tm, bar, 64 * x, in, hk, page);
       }
-      if (done + 1 < todo) page_next = look_up(in_next);
+      ++issued;
+      if (!mend) return true;
+      const bool landed = __all_sync(0xffffffffu, mbar_wait_drain(fix, fixes & 1, kSiteFix));
+      ++fixes;
+      const int end = (have + box - 1) / box * box;
+      for (int i = lane; i < (end - have) * C::kBoxes * 8; i += 32) {
+        const int r = have + i / (C::kBoxes * 8), piece = i % (C::kBoxes * 8);
+        *reinterpret_cast<uint4*>(dst + (piece >> 3) * (kTileM * 128) + r * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[slot]);
+      return landed;
+    };
+    int in_next, page_next = look_up(in_next);
+    int v_page = 0, v_in = 0, v_have = 0;  // two halves: the block whose V is still to come
+    for (int done = 0; done < todo && ok; ++done) {
+      const int in = in_next, hk = it.hk, have = it.keys - j * kBlockN;
+      const bool begins = done == 0 || j == 0, ends = j + 1 == it.units || done + 1 == todo;
+      const bool held = lane < boxes && lane * box < have;
+      int page = page_next;
+      if (done + 1 < todo) {
+        if (++j == it.units) {
+          next_item(w, it);
+          j = 0;
+        }
+        page_next = look_up(in_next);
+      }
       if ((unsigned)page >= (unsigned)p.num_pages) {
         if (held) record_bad_index(kSitePage);
         page = p.num_pages;  // out of range: zeros
       }
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {
-        const int slot = issued % S;
-        if (!mbar_wait_warp(&kv_empty[slot], ((issued / S) & 1) ^ 1u, kSiteEmpty)) {
-          ok = false;
-          break;
-        }
-        const bool mend = kv == 1 && ragged;
-        uint64_t* bar = mend ? fix : &kv_full[slot];
-        uint8_t* dst = sRing + slot * C::kTile;
-        if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
-        __syncwarp();
-        if (lane < boxes) {
-          const CUtensorMap* tm = kv ? &tmV : &tmK;
-#pragma unroll
-          for (int x = 0; x < C::kBoxes; ++x)
-            tma_load_4d(dst + x * (kTileM * 128) + lane * box * 128, tm, bar, 64 * x, in, hk, page);
-        }
-        ++issued;
-        if (mend) {
-          ok = __all_sync(0xffffffffu, mbar_wait_drain(fix, fixes & 1, kSiteFix));
-          ++fixes;
-          const int end = (have + box - 1) / box * box;
-          for (int i = lane; i < (end - have) * C::kBoxes * 8; i += 32) {
-            const int r = have + i / (C::kBoxes * 8), piece = i % (C::kBoxes * 8);
-            *reinterpret_cast<uint4*>(dst + (piece >> 3) * (kTileM * 128) + r * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_full[slot]);
-          if (!ok) break;
-        }
+      ok = copy(false, page, in, hk, have);
+      if (step == 2) {
+        if (ok && !begins) ok = copy(true, v_page, v_in, hk, v_have);
+        v_page = page, v_in = in, v_have = have;
       }
+      if (ok && (step == 1 || ends)) ok = copy(true, page, in, hk, have);
     }
     // Every copy issued must land before the block can exit.
     for (int i = (issued > S ? issued - S : 0); i < issued; ++i)
       mbar_wait_drain(&kv_full[i % S], (i / S) & 1, kSiteTeardown);
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMA issuer (whole warp)
+    // Every instruction between a softmax warp's arrival and the MMAs that answer it is on the
+    // chain of a tile's blocks, so the ring is walked by one running slot (items are taken in the
+    // order that they were loaded) and the descriptors are advanced, not built.
     bool ok = true;
     const uint64_t q_desc[2] = {sdesc_sw128(smem_u32(sQ), 16, 1024),
                                 step == 2 ? sdesc_sw128(smem_u32(sQ), 16, 1024)
                                           : sdesc_sw128(smem_u32(sQ + C::kTile), 16, 1024)};
     const uint64_t ring_k = sdesc_sw128(smem_u32(sRing), 16, 1024);
     const uint64_t ring_v = sdesc_sw128(smem_u32(sRing), kTileM * 128, 1024);
-    int base = 0;           // ring item of the share's first K
-    int cnt[2] = {0, 0};    // blocks done by tile t
-    int q_cnt[2] = {0, 0};  // items whose Q_t has been waited for
-    auto wait_item = [&](int i) {
-      const bool r = mbar_wait_warp(&kv_full[i % S], (i / S) & 1, kSiteKV);
-      tc_fence_after();
-      return r;
+    int slot = -1;
+    uint32_t par = 1;       // of the slot's phase in use
+    uint32_t p_par = 0;     // bit t: parity of tile t's next P
+    uint32_t q_par = 0;     // bit t: parity of tile t's next Q
+    auto take = [&]() {     // the next ring item
+      if (++slot == S) slot = 0;
+      if (slot == 0) par ^= 1;
+      return slot;
     };
-    auto issue_s = [&](int t, int i) {
-      const uint64_t kd = sdesc_add(ring_k, (i % S) * C::kTile);
+    auto landed = [&](int at) {
+      ok = mbar_wait_warp(&kv_full[at], par, kSiteKV);
+      tc_fence_after();
+      return ok;
+    };
+    auto issue_s = [&](int t, int at) {
+      const uint64_t kd = sdesc_add(ring_k, at * C::kTile);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const uint32_t off = (ks >> 2) * (kTileM * 128) + (ks & 3) * 32;
@@ -387,8 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_commit_warp(&s_full[t]);
     };
-    auto issue_pv = [&](int t, int i, int ks0, int ks1, bool add) {
-      const uint64_t vd = sdesc_add(ring_v, (i % S) * C::kTile);
+    auto issue_pv = [&](int t, uint64_t vd, int ks0, int ks1, bool add) {
 #pragma unroll
       for (int ks = ks0; ks < ks1; ++ks)
         mma_f16_ts_warp(tmem + C::kOCol + t * D, tmem + t * kBlockN + ks * 8, sdesc_add(vd, ks * 16 * 128), kIdescO,
@@ -397,63 +409,68 @@ __global__ void __launch_bounds__(kThreads, 1)
     Item it = first;
     int j0 = j_first;
     for (int done = 0; done < todo && ok;) {
-      const int seg = min(it.units - j0, todo - done);
+      const int seg = min(it.units - j0, todo - done), j1 = j0 + seg;
       int from[2], to[2];
-      for (int t = 0; t < 2; ++t) tile_range(it, t, j0, j0 + seg, from[t], to[t]);
-      // Ring item of K_j: base + 2 (j - j0); of V_j: one more.
-      auto k_item = [&](int j) { return base + 2 * (j - j0); };
+      for (int t = 0; t < 2; ++t) tile_range(it, t, j0, j1, from[t], to[t]);
       // Q_t is in (its softmax warps write it once the item before is done with it).
-      for (int t = 0; t < 2 && ok; ++t)
-        if (step == 2 ? t == 0 : from[t] < to[t]) ok = mbar_wait_warp(&q_full[t], q_cnt[t]++ & 1, kSiteQ);
-      tc_fence_after();
-      // K_j is waited for once and released once the last tile that takes it has issued.
-      int k_waited = j0 - 1;
-      auto need_k = [&](int j) {
-        while (ok && k_waited < j) ok = wait_item(k_item(++k_waited));
-        return ok;
-      };
-      int k_released = j0 - 1;
-      auto release_k = [&](int j) {
-        while (k_released < j) {
-          ++k_released;
-          tc_commit_warp(&kv_empty[k_item(k_released) % S]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (ok && (step == 2 ? t == 0 : from[t] < to[t])) {
+          ok = mbar_wait_warp(&q_full[t], (q_par >> t) & 1, kSiteQ);
+          q_par ^= 1u << t;
         }
-      };
-      for (int t = 0; t < 2 && ok; ++t)
-        if (from[t] < to[t] && need_k(from[t])) issue_s(t, k_item(from[t]));
-      if (ok) release_k(min(j0 + seg - 1, j0 + step - 1));
-      for (int j = j0; j < j0 + seg && ok; ++j) {
-        bool v_in = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j < from[t] || j >= to[t] || (step == 2 && ((j ^ from[t]) & 1))) continue;
-          if (!v_in) {
-            if (!(ok = wait_item(k_item(j) + 1))) break;
-            v_in = true;
-          }
-          const bool add = j > from[t];
-          if (!(ok = mbar_wait_warp(&p_half[t], cnt[t] & 1, kSiteP))) break;
+      tc_fence_after();
+      // The first S of each tile.
+      for (int i = 0; i < min(step, seg) && ok; ++i) {
+        const int at = take();
+        if (!landed(at)) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (from[t] == j0 + i && from[t] < to[t]) issue_s(t, at);
+        tc_commit_warp(&kv_empty[at]);
+      }
+#pragma unroll 1
+      for (int j = j0; j < j1 && ok; ++j) {
+        // V_j, and K of the block that its tiles take next.
+        const int v_at = take();
+        if (!landed(v_at)) break;
+        const uint64_t vd = sdesc_add(ring_v, v_at * C::kTile);
+        const bool more = j + step < j1;
+        int k_at = 0;
+        bool k_in = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || j < from[t] || j >= to[t] || (step == 2 && ((j ^ t) & 1))) continue;
+          const uint32_t pp = (p_par >> t) & 1;
+          p_par ^= 1u << t;
+          if (!(ok = mbar_wait_warp(&p_half[t], pp, kSiteP))) break;
           tc_fence_after();
-          issue_pv(t, k_item(j) + 1, 0, kBlockN / 32, add);
-          if (!(ok = mbar_wait_warp(&p_full[t], cnt[t] & 1, kSiteP))) break;
+          issue_pv(t, vd, 0, kBlockN / 32, j > from[t]);
+          if (!(ok = mbar_wait_warp(&p_full[t], pp, kSiteP))) break;
           tc_fence_after();
-          issue_pv(t, k_item(j) + 1, kBlockN / 32, kBlockN / 16, add);
-          ++cnt[t];
+          issue_pv(t, vd, kBlockN / 32, kBlockN / 16, j > from[t]);
           if (j + step < to[t]) {
-            if (!need_k(j + step)) break;
-            issue_s(t, k_item(j + step));
+            // Behind PV_t(j) in issue order: S_t overwrites P_t only once that has read it.
+            if (!k_in) {
+              k_at = take();
+              k_in = true;
+              if (!landed(k_at)) break;
+            }
+            issue_s(t, k_at);
           } else {
             tc_commit_warp(&o_full[t]);
           }
         }
         if (!ok) break;
-        if (!v_in) ok = wait_item(k_item(j) + 1);  // no tile takes V_j: its slot is free again
-        if (!ok) break;
-        tc_commit_warp(&kv_empty[(k_item(j) + 1) % S]);
-        const int k_next = min(j + step, j0 + seg - 1);
-        if (!need_k(k_next)) break;
-        release_k(k_next);
+        tc_commit_warp(&kv_empty[v_at]);
+        if (more) {
+          if (!k_in) {  // no tile takes it
+            k_at = take();
+            if (!landed(k_at)) break;
+          }
+          tc_commit_warp(&kv_empty[k_at]);
+        }
       }
-      base += 2 * seg;
       done += seg;
       j0 = 0;
       if (done < todo) next_item(w, it);
@@ -468,19 +485,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = tmem + lane_off + t * kBlockN;
     const uint32_t o_tmem = tmem + lane_off + C::kOCol + t * D;
     bool ok = true;
-    int cnt = 0, o_cnt = 0, meets = 0;
+    uint32_t phase = 0;  // parities of the waits for s_full (bit 0), o_full (1) and meet_bar (2)
     auto meet = [&]() {  // a bounded barrier of the softmax warps
       __syncwarp();
       if (lane == 0) mbar_arrive(meet_bar);
-      return mbar_wait_warp(meet_bar, meets++ & 1, kSiteMeet);
+      const bool r = mbar_wait_warp(meet_bar, (phase >> 2) & 1, kSiteMeet);
+      phase ^= 4;
+      return r;
     };
     volatile Walk* walk = walks + warp;
     if (lane == 0) {
       walk->it.b = first.b, walk->it.hk = first.hk, walk->it.pair = first.pair;
       walk->it.units = first.units, walk->it.keys = first.keys, walk->it.visible = first.visible;
-      walk->j0 = j_first, walk->done = 0, walk->todo = todo, walk->c = c, walk->line_id = line_id, walk->nc = line.nc;
+      walk->j0 = j_first, walk->done = 0, walk->todo = todo, walk->c = c, walk->line_id = line_id;
       walk->item = !w.prefix_pass ? 0 : (w.lines > 1 ? first.hk : first.hk * w.pairs + first.pair);
-      walk->unit = u0, walk->units = line.units;
+      walk->unit = u0;
+      walk->line.q = line.q, walk->line.more = line.more, walk->line.nc = line.nc;
     }
     __syncwarp();
     auto item_now = [&]() {
@@ -496,30 +516,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                                        ((((col >> 2) & 7) ^ (row & 7)) << 4));
     };
     while (ok && walk->done < walk->todo) {
-      int from, to, lim, tile_sees;
-      bool warp_live;
+      int from, to, lim;
       {
         const Item it = item_now();
         const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done);
         tile_range(it, t, j0, j0 + seg, from, to);
-        const int64_t row_begin = tile_rows_begin(it, t), row = row_begin + r;
+        const int row_begin = tile_rows_begin(it, t), row = row_begin + r;
         const bool live = row < w.rows;
-        warp_live = row_begin + quad * 32 < w.rows;
         const Row at = query_row(w, it, live ? row : 0);
-        // Keys that this row sees, and that every row of the tile does.
-        lim = !live ? 0 : (w.prefix_pass ? it.keys : max(0, it.keys - p.n + at.i + 1));
-        tile_sees = w.prefix_pass ? it.keys : max(0, it.keys - p.n + 1 + (int)(min(row_begin, w.rows - 1) / p.G));
+        // Keys that this row sees; -1 in a warp without a query.
+        lim = row_begin + quad * 32 >= w.rows ? -1 : !live ? 0 : (w.prefix_pass ? it.keys : max(0, it.keys - p.n + at.i + 1));
         // Q_t is written for every share that its MMAs take part in.  (With two halves both tiles
         // read Q_0, and the halves meet at the end of each item, so it is idle here.)
         if (step == 2 ? t == 0 : from < to) {
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at.b * p.q_sb +
-                                                            at.i * p.q_ss + at.head * p.q_sh);
-          uint8_t* dst = sQ + t * C::kTile + r * 128;
-#pragma unroll
-          for (int x = 0; x < D / 8; ++x) {
-            const uint4 v = live && x * 8 < p.D ? src[x] : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(dst + (x >> 3) * (kTileM * 128) + (((x & 7) ^ (r & 7)) << 4)) = v;
+          // A warp copies its 32 rows, whole rows at a time; all the copies are in flight at once (a
+          // round trip to memory is over a microsecond here, and this one is on the way of every
+          // share).
+          constexpr int kPieces = D / 8;  // 16-byte pieces of a row
+          const int piece = lane % kPieces;
+#pragma unroll 4
+          for (int x = lane / kPieces; x < 32; x += 32 / kPieces) {
+            const int tile_row = quad * 32 + x;
+            const bool in = row_begin + tile_row < w.rows && piece * 8 < p.D;
+            const Row from_q = query_row(w, it, in ? row_begin + tile_row : 0);
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + (in ? from_q.b * p.q_sb + from_q.i * p.q_ss +
+                                                                                from_q.head * p.q_sh + piece * 8
+                                                                          : 0);
+            cp16(smem_u32(sQ + t * C::kTile + (piece >> 3) * (kTileM * 128) + tile_row * 128) +
+                     (((piece & 7) ^ (tile_row & 7)) << 4),
+                 src, in);
           }
+          cp_commit();
+          cp_wait<0>();
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_full[t]);
@@ -527,36 +555,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const bool any = from < to;
       float m_used = -INFINITY, l = 0.f;
-      bool begun = false;
+      if (lim < 0) {  // no query in this warp's rows: what P holds there reaches no result
 #pragma unroll 1
-      for (int j = from; j < to; j += step) {
-        if (!mbar_wait_warp(&s_full[t], cnt & 1, kSiteS)) {
-          ok = false;
-          break;
-        }
-        ++cnt;
-        tc_fence_after();
-        if (!warp_live) {  // no query in this warp's rows: what P holds there reaches no result
-          if (lane == 0) {
+        for (int j = from; j < to && ok; j += step) {
+          ok = mbar_wait_warp(&s_full[t], phase & 1, kSiteS);
+          phase ^= 1;
+          if (ok && lane == 0) {
             mbar_arrive(&p_half[t]);
             mbar_arrive(&p_full[t]);
           }
-          continue;
         }
+        from = to;
+      }
+#pragma unroll 1
+      for (int j = from; j < to; j += step) {
+        if (!mbar_wait_warp(&s_full[t], phase & 1, kSiteS)) {
+          ok = false;
+          break;
+        }
+        phase ^= 1;
+        tc_fence_after();
         uint32_t sr[kBlockN];
         const int n0 = j * kBlockN;
 #pragma unroll
         for (int x = 0; x < kBlockN / 32; ++x) tmem_ld32(s_tmem + x * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[x * 32]));
         tmem_wait_ld();
-        if (n0 + kBlockN > tile_sees && n0 + kBlockN > lim) {
+        if (n0 + kBlockN > lim) {
 #pragma unroll
           for (int x = 0; x < kBlockN; ++x)
             if (n0 + x >= lim) sr[x] = __float_as_uint(-INFINITY);
         }
         const float m_new = row_max<kBlockN>(sr) * p.scale_log2;
         const bool need = m_new > m_used + kLazy;
-        const bool warp_rescale = __any_sync(0xffffffffu, need) && begun;
-        begun = true;
+        // A row without a maximum so far holds nothing (in its first block, not even O).
+        const bool warp_rescale = __any_sync(0xffffffffu, need && m_used != -INFINITY);
         float alpha = 1.f;
         if (need) {
           alpha = fa::ex2(m_used - m_new);  // 0 where m_used is -inf
@@ -611,8 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (any) {
-        if (!(ok = mbar_wait_warp(&o_full[t], o_cnt & 1, kSiteO))) break;
-        ++o_cnt;
+        if (!(ok = mbar_wait_warp(&o_full[t], (phase >> 1) & 1, kSiteO))) break;
+        phase ^= 2;
         tc_fence_after();
       }
       // A row that saw no key has m = -inf (its l is of the 2^-125 that the polynomial gives for
@@ -624,14 +656,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_now();
       const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done), item = walk->item;
       Line ln;
-      ln.nc = walk->nc, ln.units = walk->units;
-      const int64_t item0 = walk->unit - j0;
+      ln.q = walk->line.q, ln.more = walk->line.more, ln.nc = walk->line.nc;
+      const int item0 = walk->unit - j0;
       const int me = walk->c, cf = ln.block_of(item0), cl = ln.block_of(item0 + it.units - 1);
-      // A whole item is written at once; a part of one, and what a prefix's shares join, is left
-      // as a share in the workspace.
-      const bool direct = !w.prefix_pass && cf == cl && !p.pre.slots;
-      const int64_t row_begin = tile_rows_begin(it, step == 2 ? 0 : t);
-      const int quad_rows = (int)max((int64_t)0, min((int64_t)32, w.rows - row_begin - quad * 32));  // queries among this warp's rows
+      // A whole item is written at once; a part of one is left as a share in the workspace.
+      const bool direct = !w.prefix_pass && cf == cl;
+      const int row_begin = tile_rows_begin(it, step == 2 ? 0 : t);
+      const int quad_rows = max(0, min(32, w.rows - row_begin - quad * 32));  // queries among this warp's rows
       auto slot_of = [&](int x) {
         return w.prefix_pass ? prefix_slot<D>(p.pre, p.Hk, walk->line_id, item, x)
                              : p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kSlotFloats<D>;
@@ -664,13 +695,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         w0 = w1 = m_used == -INFINITY ? 0.f : 1.f;
       }
       const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);
-      const float scale = direct ? inv : 1.f;
+      const float scale = direct && !p.row_share ? inv : 1.f;
       w0 *= scale, w1 *= scale;
       float* share = direct ? nullptr : slot_of(me);
       if (quad_rows > 0) {
         if (c0 == 0 && lane < quad_rows) {
           if (!direct) {
             *reinterpret_cast<float2*>(share + kWideRows * D + 2 * (t * kTileM + r)) = make_float2(m_row, l_row);
+          } else if (p.row_share) {
+            const Row at = query_row(w, it, row_begin + r);
+            *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * D +
+                                       2 * (int64_t)((at.b * p.n + at.i) * p.H + at.head)) = make_float2(m_row, l_row);
           } else if (p.lse) {
             const Row at = query_row(w, it, row_begin + r);
             p.lse[((int64_t)at.b * p.n + at.i) * p.H + at.head] = l_row == 0.f ? -INFINITY : (m_row + log2f(l_row)) * kLn2;
@@ -706,7 +741,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           }
           __syncwarp();
-          if (!direct) {  // 4 values a lane, whole rows of D / 2 values
+          if (direct && p.row_share) {  // 4 values a lane, whole rows of D / 2 values
+            constexpr int kLanes = D / 8;
+            const int col = lane % kLanes * 4;
+#pragma unroll 2
+            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes) {
+              const Row at = query_row(w, it, row_begin + quad * 32 + rr);
+              *reinterpret_cast<float4*>(p.row_share + (int64_t)((at.b * p.n + at.i) * p.H + at.head) * D + cb + col) =
+                  *stage_at(quad * 32 + rr, col);
+            }
+          } else if (!direct) {
             constexpr int kLanes = D / 8;
             const int col = lane % kLanes * 4;
             float* dst = share + (step == 2 ? 0 : t * kTileM) * D + cb + col;
@@ -743,21 +787,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = meet())) break;
         if (*s_last) {
           __threadfence();
-          if (p.pre.slots) griddep_wait();  // the prefix's shares are complete
           constexpr int kLanes = D / 4;  // 4 values a lane
           const int col = lane % kLanes * 4;
-          // With two halves the tiles' warps share the rows of a quadrant.
-          const int first_row = step == 2 ? t * 16 : 0, end_row = min(quad_rows, step == 2 ? first_row + 16 : 32);
+          const int item_begin = tile_rows_begin(it, 0), item_rows = min(step == 2 ? kTileM : 2 * kTileM, w.rows - item_begin);
 #pragma unroll 1
-          for (int rr = first_row + lane / kLanes; rr < end_row; rr += 32 / kLanes) {
-            const int tile_row = (step == 2 ? 0 : t * kTileM) + quad * 32 + rr;
-            const Row at = query_row(w, it, row_begin + quad * 32 + rr);
+          for (int tile_row = warp * (32 / kLanes) + lane / kLanes; tile_row < item_rows; tile_row += 8 * (32 / kLanes)) {
+            const Row at = query_row(w, it, item_begin + tile_row);
             float mm = -INFINITY, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
             join_shares<D, 4, 4>(
                 cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kWideRows, tile_row, col, mm, ll, v);
-            if (p.pre.slots)
-              join_prefix<D, 4, 4>(p.pre, p.Hk, it.hk, (int64_t)at.b * p.rows + (int64_t)at.i * p.G + at.head - it.hk * p.G, col,
-                                   mm, ll, v);
+            if (p.row_share) {
+              leave_row<D, 4>(p, (at.b * p.n + at.i) * p.H + at.head, col, mm, ll, v);
+              continue;
+            }
             const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
             if (col < p.D)
               *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh + col) =
@@ -789,6 +831,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, 512);
+  // The join of the prefix's shares waits for this kernel, and so for the prefix pass before it.
+  if (!w.prefix_pass && p.row_share) griddep_wait();
 }
 
 template <int D, bool kBf16>
@@ -827,7 +871,7 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   WideParams w{};
   w.p = p;
   w.prefix_pass = prefix_pass;
-  w.rows = prefix_pass ? (int64_t)p.B * p.rows : p.rows;
+  w.rows = prefix_pass ? p.B * p.rows : p.rows;
   w.halves = w.rows <= kTileM ? 2 : 1;
   const int64_t tile = w.halves == 2 ? kTileM : 2 * kTileM;
   w.pairs = (int)((w.rows + tile - 1) / tile);
@@ -843,7 +887,7 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   CUtensorMap tk, tv;
   if (int st = page_map(&tk, bf16, p.k, p, p.k_sp, p.k_ss, p.k_sh, w.box_rows)) return st;
   if (int st = page_map(&tv, bf16, p.v, p, p.v_sp, p.v_ss, p.v_sh, w.box_rows)) return st;
-  const bool dependent = !prefix_pass && p.pre.slots != nullptr;
+  const bool dependent = !prefix_pass && p.row_share != nullptr;
   if (p.D > 64)
     return bf16 ? launch<128, true>(tk, tv, w, (int)grid, dependent, s) : launch<128, false>(tk, tv, w, (int)grid, dependent, s);
   return bf16 ? launch<64, true>(tk, tv, w, (int)grid, dependent, s) : launch<64, false>(tk, tv, w, (int)grid, dependent, s);
