@@ -22,11 +22,8 @@
 // end then holds up one warp, not four).
 #include <atomic>
 
-#include <cstdlib>
 #include "lk_abi.h"
 #include "paged_common.cuh"
-static int64_t many_items() { const char* e = getenv("LK_MI"); return e ? atoll(e) : 256; }
-static int64_t prefix_pass() { const char* e = getenv("LK_PT"); return e ? atoll(e) : 1024; }
 
 namespace lk {
 namespace paged {
@@ -121,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const int per_seq = p.Hk * tiles;
   const int c = blockIdx.x * kTeams + warp / kTeam;  // this warp's team
   Line line;
-  if (!locate<kThreads, kTeams>(p.B, gridDim.x * kTeams, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
+  if (!locate<kThreads, kTeams>(p.B, gridDim.x * kTeams, 1, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
                                 [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; }))
     return;
   if (c >= line.nc) return;
@@ -379,11 +376,23 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
       }
       if (last) {
         __threadfence();
+        // A team of four warps has as many rows in flight as one warp alone, in fewer steps.
+        constexpr int kR = kTeam == 1 ? 4 : 1, kBatch = kTeam == 1 ? 3 : 8;
 #pragma unroll 1
-        for (int row = in_team; row < rows_here; row += kTeam) {
-          float mm = -INFINITY, ll = 0.f, v[kPer] = {};
-          join_shares<DP, kPer, 8>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, row, col, mm, ll, v);
-          write_out(row, mm, ll, v);
+        for (int row0 = in_team * kR; row0 < rows_here; row0 += kTeam * kR) {
+          int r[kR];
+          float mm[kR], ll[kR], v[kR][kPer];
+#pragma unroll
+          for (int k = 0; k < kR; ++k) {
+            r[k] = min(row0 + k, rows_here - 1);
+            mm[k] = -INFINITY, ll[k] = 0.f;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+          }
+          join_shares<DP, kPer, kR, kBatch>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, r, 0, col, mm, ll, v);
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+            if (row0 + k < rows_here) write_out(row0 + k, mm[k], ll[k], v[k]);
         }
         if (lane == 0 && in_team == 0) p.counters[cf] = 0;
       }
@@ -411,11 +420,13 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const Params p) {
   const int token = row / p.H, head = row - token * p.H, b = token / p.n, i = token - b * p.n;
   const int hk = p.by_G.div(head), col = lane * kPer;
   using V = typename std::conditional<kPer % 4 == 0, float4, float2>::type;
-  float v[kPer];
+  float v1[1][kPer];
+  float(&v)[kPer] = v1[0];
   *reinterpret_cast<V*>(v) = __ldcg(reinterpret_cast<const V*>(p.row_share + (int64_t)row * DP + col));
   const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row));
-  float mm = ml.x, ll = ml.y;
-  join_prefix<DP, kPer, 8>(p.pre, p.Hk, hk, b * p.rows + i * p.G + head - hk * p.G, col, mm, ll, v);
+  float m1[1] = {ml.x}, l1[1] = {ml.y};
+  join_prefix<DP, kPer, 8>(p.pre, p.Hk, hk, b * p.rows + i * p.G + head - hk * p.G, col, m1, l1, v1);
+  const float mm = m1[0], ll = l1[0];
   const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
   if (col < p.D) {
     uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o_sb + i * p.o_ss + head * p.o_sh + col;
@@ -457,7 +468,7 @@ int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
 template <int DP, bool kBf16>
 int launch_rows16(const Params& p, int64_t keys, cudaStream_t s) {
   const int64_t items = (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows);
-  return items >= many_items() ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
+  return items >= kManyItems ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
 }
 
 }  // namespace paged
@@ -478,6 +489,9 @@ PrefixShares prefix_shares(int64_t rows, int64_t H_kv, int64_t prefix) {
   const int64_t items = s.lines > 1 ? H_kv : H_kv * s.pairs;
   s.nc = sms / s.lines;
   if (s.nc > items * s.units) s.nc = (int)(items * s.units);
+  // As few blocks as leave the longest share as it is: the SMs that are free run the sequences' own keys.
+  const int64_t longest = (items * s.units + s.nc - 1) / s.nc;
+  s.nc = (int)((items * s.units + longest - 1) / longest);
   return s;
 }
 int64_t prefix_floats(const PrefixShares& s, int64_t H_kv, int64_t DP) {
@@ -554,7 +568,7 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   const int64_t DP = D > 64 ? 128 : 64;
   bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
   for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
-  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > prefix_pass()) {
+  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
     paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
     if ((int64_t)pre.units * H_kv * pre.pairs > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
     pre.slots = p.partial + paged::own_floats(p.rows, DP);

@@ -57,7 +57,7 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
-constexpr int kCounters = 4096;  // ints at the workspace's start: one per block, zero between calls
+constexpr int kCounters = 4096;  // ints at the workspace's start: one per team or warp, zero between calls
 constexpr float kLn2 = 0.69314718055994531f;
 
 // Where the shares of a shared prefix lie that the 256-row kernel left (paged_wide.cu): its
@@ -135,11 +135,12 @@ struct Line {
 
 // Finds where a block's teams (kTeams of them, consecutive on the line from team `team0`) begin, by
 // the whole block: units_of(b) is sequence b's count of units in 64 bits.  Two passes over the lengths: their
-// sum, by which the line is cut into `teams`, and a scan up to the places looked for.  found[i] =
+// sum, by which the line is cut into `teams` (fewer, where that leaves them under `least` units: a
+// share costs its join), and a scan up to the places looked for.  found[i] =
 // (sequence, unit among the sequence's) for team i.  Returns false (reported) if the line does not
 // fit 31 bits, which takes 2^37 keys.  scratch: 8-byte aligned, kThreads / 32 values.
 template <int kThreads, int kTeams, class UnitsOf>
-__device__ __forceinline__ bool locate(int B, int teams, int team0, long long* scratch, int2* found, Line& line,
+__device__ __forceinline__ bool locate(int B, int teams, int least, int team0, long long* scratch, int2* found, Line& line,
                                        UnitsOf units_of) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -157,7 +158,7 @@ __device__ __forceinline__ bool locate(int B, int teams, int team0, long long* s
     record_bad_index(kSiteLength);
     return false;
   }
-  line.cut((int)all, teams);
+  line.cut((int)all, min(teams, max(1, (int)all / least)));
   const int last = line.begin(min(team0 + kTeams, line.nc) - 1);  // the last place looked for
   int base = 0;
   for (int b0 = 0; b0 < B && base <= last; b0 += kThreads) {
@@ -199,39 +200,49 @@ __device__ __forceinline__ float* prefix_slot(const PrefixShares& s, int Hk, int
   return s.slots + (line * per_line + item + block) * kSlotFloats<DP>;
 }
 
-// Joins n shares (slot(x) is the x-th; slots of `rows` rows) of row r, columns d .. d + kPer, to the
-// sums (mm, ll, v), kBatch loads at a time: a share after the other, the load latencies would add up.
-template <int DP, int kPer, int kBatch, class Slot>
-__device__ __forceinline__ void join_shares(int n, Slot slot, int rows, int r, int d, float& mm, float& ll, float (&v)[kPer]) {
+// Joins n shares (slot(x) is the x-th; slots of `rows` rows), columns d .. d + kPer of rows r[0 .. kR)
+// (whose (m, l) is that of row r + ml_off), to the sums (mm, ll, v) of each.  kR kBatch loads are in flight at a time: a round trip to memory
+// takes over a microsecond, so one share of one row after the other is what a join must not do.
+template <int DP, int kPer, int kR, int kBatch, class Slot>
+__device__ __forceinline__ void join_shares(int n, Slot slot, int rows, const int (&r)[kR], int ml_off, int d, float (&mm)[kR], float (&ll)[kR],
+                                            float (&v)[kR][kPer]) {
   using V = typename std::conditional<kPer % 4 == 0, float4, float2>::type;
   constexpr int kW = sizeof(V) / 4;
 #pragma unroll 1
   for (int x0 = 0; x0 < n; x0 += kBatch) {
-    float2 ml[kBatch];
-    V f[kBatch][kPer / kW];
+    float2 ml[kBatch][kR];
+    V f[kBatch][kR][kPer / kW];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const float* s = slot(min(x0 + i, n - 1));
-      ml[i] = __ldcg(reinterpret_cast<const float2*>(s + rows * DP + 2 * r));
 #pragma unroll
-      for (int e = 0; e < kPer / kW; ++e) f[i][e] = __ldcg(reinterpret_cast<const V*>(s + r * DP + d + kW * e));
-      if (x0 + i >= n) ml[i].x = -INFINITY;
+      for (int k = 0; k < kR; ++k) {
+        ml[i][k] = __ldcg(reinterpret_cast<const float2*>(s + rows * DP + 2 * (r[k] + ml_off)));
+#pragma unroll
+        for (int e = 0; e < kPer / kW; ++e) f[i][k][e] = __ldcg(reinterpret_cast<const V*>(s + r[k] * DP + d + kW * e));
+      }
     }
-    float top = mm;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
-    const float a = weight(mm, top);
-    mm = top;
-    ll *= a;
+    for (int k = 0; k < kR; ++k) {
+      float top = mm[k];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] *= a;
+      for (int i = 0; i < kBatch; ++i) {
+        if (x0 + i >= n) ml[i][k].x = -INFINITY;
+        top = fmaxf(top, ml[i][k].x);
+      }
+      const float a = weight(mm[k], top);
+      mm[k] = top;
+      ll[k] *= a;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (ml[i].x == -INFINITY) continue;  // no key: its O may not have been written
-      const float b = weight(ml[i].x, top);
-      ll += b * ml[i].y;
+      for (int e = 0; e < kPer; ++e) v[k][e] *= a;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) v[e] += b * reinterpret_cast<const float*>(&f[i][e / kW])[e % kW];
+      for (int i = 0; i < kBatch; ++i) {
+        if (ml[i][k].x == -INFINITY) continue;  // no key: its O may not have been written
+        const float b = weight(ml[i][k].x, top);
+        ll[k] += b * ml[i][k].y;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[k][e] += b * reinterpret_cast<const float*>(&f[i][k][e / kW])[e % kW];
+      }
     }
   }
 }
@@ -249,15 +260,15 @@ __device__ __forceinline__ void leave_row(const Params& p, int row, int d, float
 
 // Adds the prefix's shares for query row `row` (of all the batch's rows of K/V head hk).
 template <int DP, int kPer, int kBatch>
-__device__ __forceinline__ void join_prefix(const PrefixShares& s, int Hk, int hk, int row, int d, float& mm, float& ll,
-                                            float (&v)[kPer]) {
-  const int pair = s.tile == kWideRows ? row / kWideRows : row / (kWideRows / 2), r = row - pair * s.tile;
+__device__ __forceinline__ void join_prefix(const PrefixShares& s, int Hk, int hk, int row, int d, float (&mm)[1], float (&ll)[1],
+                                            float (&v)[1][kPer]) {
+  const int pair = s.tile == kWideRows ? row / kWideRows : row / (kWideRows / 2), r[1] = {row - pair * s.tile};
   const int line = s.lines > 1 ? pair : 0, item = s.lines > 1 ? hk : hk * s.pairs + pair;
   Line l;
   l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), s.nc);
   const int cf = l.block_of(item * s.units), cl = l.block_of((item + 1) * s.units - 1);
-  join_shares<DP, kPer, kBatch>(
-      cl - cf + 1, [&](int x) { return prefix_slot<DP>(s, Hk, line, item, cf + x); }, kWideRows, r, d, mm, ll, v);
+  join_shares<DP, kPer, 1, kBatch>(
+      cl - cf + 1, [&](int x) { return prefix_slot<DP>(s, Hk, line, item, cf + x); }, kWideRows, r, 0, d, mm, ll, v);
 }
 
 // Launches `kern`; `dependent`: as a programmatic dependent of the launch before it (it calls

@@ -40,6 +40,7 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTileM = 128;
 constexpr int kBlockN = 128;  // keys of a unit
+constexpr int kLeast = 4;     // units that a block's share has at least, where there are as many
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 
 enum WideSite : int {
@@ -153,9 +154,171 @@ __device__ __forceinline__ float row_max(const uint32_t (&sr)[n]) {
   return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
+// What a softmax warp hands on of an item.
+template <int D>
+struct HandOn {
+  const WideParams* w;
+  Item it;
+  uint8_t* sQ;
+  uint32_t tmem;
+  float m_row, l_row;   // of this thread's row
+  float w0, w1;         // weights of O_0 and O_1 in it
+  bool any0, any1;      // whether O_0 and O_1 hold anything
+  int row_begin;        // first query row of the tile
+  int quad_rows;        // queries among the warp's 32 rows
+  int cf, cl, me;       // blocks that share the item, first and last, and this one
+  __device__ __forceinline__ float* slot_of(int x) const {  // of a sequence's own keys
+    return w->p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kSlotFloats<D>;
+  }
+};
+
+// Hands on this warp's rows (with two halves, half of their columns): into `share`, or (nullptr)
+// joined with the others' shares as the result.  What a row needs once (weights, addresses) its
+// thread works out; values go through shared memory, from a row per thread to whole rows per warp.
+template <int D, bool kBf16>
+__device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int lane, int warp) {
+  using C = Cfg<D>;
+  const WideParams& w = *h.w;
+  const Params& p = w.p;
+  const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+  const bool halves = w.halves == 2, two = h.cl - h.cf == 1;
+  const int quad_rows = h.quad_rows, c0 = halves ? t * (D / 2) : 0, c1 = halves ? c0 + D / 2 : D;
+  const uint32_t o_tmem = h.tmem + ((uint32_t)(quad * 32) << 16) + C::kOCol;
+  // Row r of the tile, columns 4 .. of 32 in 32 bits, in this warp's own rows of the tile's Q buffer
+  // (128-byte swizzle).
+  auto stage_at = [&](int row, int col) {
+    return reinterpret_cast<float4*>(h.sQ + t * C::kTile + (col >> 5) * (kTileM * 128) + row * 128 +
+                                     ((((col >> 2) & 7) ^ (row & 7)) << 4));
+  };
+  // The slot's row of O of this warp's first row, and the slot's place of its (m, l) (with two halves
+  // each tile's warps leave one, for their own columns).
+  const int o_row = (halves ? 0 : t * kTileM) + quad * 32, ml_at = kWideRows * D + 2 * (t * kTileM + r);
+  // Shares to read: none, the other of two, or all (this warp's own among them).
+  const int others = share || w.prefix_pass || h.cf == h.cl ? 0 : (two ? 1 : h.cl - h.cf + 1);
+  auto other = [&](int x) { return h.slot_of(two ? h.cf + h.cl - h.me : h.cf + x); };
+  auto other_ml = [&](int x) { return __ldcg(reinterpret_cast<const float2*>(other(min(x, others - 1)) + ml_at)); };
+  const bool with_own = others < 2;
+  float mm = with_own ? h.m_row : -INFINITY, ll = with_own ? h.l_row : 0.f;
+#pragma unroll 1
+  for (int x0 = 0; x0 < others; x0 += 4) {  // four round trips to memory at a time
+    float2 ml[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) ml[x] = other_ml(x0 + x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (x0 + x >= others) break;
+      const float top = fmaxf(mm, ml[x].x);
+      ll = __fadd_rn(__fmul_rn(ll, weight(mm, top)), __fmul_rn(ml[x].y, weight(ml[x].x, top)));
+      mm = top;
+    }
+  }
+  const float inv = share || p.row_share ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
+  const float own = !with_own ? 0.f : others ? weight(h.m_row, mm) * inv : inv;
+  const float f0 = h.w0 == 0.f ? 0.f : h.w0 * own, f1 = h.w1 == 0.f ? 0.f : h.w1 * own;
+  uint64_t to = 0;  // where this thread's row goes
+  if (lane < quad_rows) {
+    if (share) {
+      *reinterpret_cast<float2*>(share + ml_at) = make_float2(mm, ll);
+      to = reinterpret_cast<uint64_t>(share + (int64_t)(o_row + lane) * D);
+    } else {
+      const Row at = query_row(w, h.it, h.row_begin + r);
+      const int64_t out_row = ((int64_t)at.b * p.n + at.i) * p.H + at.head;
+      if (p.row_share) {
+        to = reinterpret_cast<uint64_t>(p.row_share + out_row * D);
+        if (c0 == 0)
+          *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * D + 2 * out_row) = make_float2(mm, ll);
+      } else {
+        to = reinterpret_cast<uint64_t>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh);
+        if (p.lse && c0 == 0) p.lse[out_row] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+      }
+    }
+  }
+#pragma unroll 1
+  for (int cb = c0; cb < c1; cb += D / 2) {
+#pragma unroll 1
+    for (int x = 0; x < D / 64; ++x) {
+      uint32_t ov[32];
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      if (h.any0) {
+        tmem_ld32(o_tmem + cb + x * 32, ov);
+        tmem_wait_ld();
+        if (f0 != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = f0 * __uint_as_float(ov[i]);
+        }
+      }
+      __syncwarp();
+      if (h.any1) {
+        tmem_ld32(o_tmem + D + cb + x * 32, ov);
+        tmem_wait_ld();
+        if (f1 != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += f1 * __uint_as_float(ov[i]);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+    __syncwarp();
+    constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes;  // 4 columns a lane
+    const int col = lane % kLanes * 4, sub = lane / kLanes;
+#pragma unroll 1
+    for (int x = 0; x < others; ++x) {
+      const float f = weight(other_ml(x).x, mm) * inv;
+      const float* src = other(x) + (int64_t)o_row * D + cb + col;
+#pragma unroll 1
+      for (int r0 = 0; r0 < quad_rows; r0 += 8 * kRowsPer) {  // eight loads in flight
+        float4 g[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          g[k] = __ldcg(reinterpret_cast<const float4*>(src + min(r0 + k * kRowsPer + sub, quad_rows - 1) * D));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rr = r0 + k * kRowsPer + sub;
+          const float fr = __shfl_sync(~0u, f, rr & 31);
+          if (rr >= quad_rows || fr == 0.f) continue;  // a share without a key may not hold O
+          float4* at = stage_at(quad * 32 + rr, col);
+          float4 a = *at;
+          // Products rounded before the sum: of two shares it is then the same both ways round.
+          a.x = __fadd_rn(a.x, __fmul_rn(fr, g[k].x)), a.y = __fadd_rn(a.y, __fmul_rn(fr, g[k].y));
+          a.z = __fadd_rn(a.z, __fmul_rn(fr, g[k].z)), a.w = __fadd_rn(a.w, __fmul_rn(fr, g[k].w));
+          *at = a;
+        }
+      }
+      __syncwarp();
+    }
+    if (share || p.row_share) {
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += kRowsPer) {
+        const int rr = r0 + sub;
+        float* dst = reinterpret_cast<float*>(__shfl_sync(~0u, to, rr));
+        if (rr < quad_rows) *reinterpret_cast<float4*>(dst + cb + col) = *stage_at(quad * 32 + rr, col);
+      }
+    } else {
+      constexpr int kLanes8 = D / 16, kRows8 = 32 / kLanes8;  // 8 columns a lane
+      const int col8 = lane % kLanes8 * 8;
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += kRows8) {
+        const int rr = r0 + lane / kLanes8;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(__shfl_sync(~0u, to, rr));
+        if (rr < quad_rows && cb + col8 < p.D) {
+          const float4 a = *stage_at(quad * 32 + rr, col8), b = *stage_at(quad * 32 + rr, col8 + 4);
+          *reinterpret_cast<uint4*>(dst + cb + col8) =
+              make_uint4(pack2<kBf16>(a.x, a.y), pack2<kBf16>(a.z, a.w), pack2<kBf16>(b.x, b.y), pack2<kBf16>(b.z, b.w));
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WideParams w) {
+    paged_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const __grid_constant__ WideParams w) {
   using C = Cfg<D>;
   constexpr int S = C::kStages;
   constexpr uint32_t kIdescS = make_idesc(1, kBf16 ? 1 : 0, kBf16 ? 1 : 0, 0, 0, kTileM, kBlockN);
@@ -178,8 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* meet_bar = fix + 1;      // [1]  the eight softmax warps meet
   uint64_t* drain = meet_bar + 1;    // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  int* s_last = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile Walk* walks = reinterpret_cast<volatile Walk*>(s_last + 1);  // [8] of the softmax warps
+  volatile Walk* walks = reinterpret_cast<volatile Walk*>(drain + 2);  // [8] of the softmax warps
   long long* scratch = reinterpret_cast<long long*>(sQ);  // before the pipeline starts
 
   const int warp = warp_id();
@@ -220,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int x = 0; x < w.pairs; ++x) sum += units_of_keys(visible_keys(w, L, x));
       return sum;
     };
-    if (!locate<kThreads, 1>(p.B, gridDim.x, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; }))
+    if (!locate<kThreads, 1>(p.B, gridDim.x, kLeast, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; }))
       return;
     if (c >= line.nc) return;
     first.b = found->x;
@@ -509,15 +671,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       i.units = walk->it.units, i.keys = walk->it.keys, i.visible = walk->it.visible;
       return i;
     };
-    // Row r of the tile, columns 32 x .. 32 x + 31 in 32 bits, in this warp's own rows of the
-    // tile's Q buffer (128-byte swizzle): O's way from a thread per row to whole rows.
-    auto stage_at = [&](int row, int col) {
-      return reinterpret_cast<float4*>(sQ + t * C::kTile + (col >> 5) * (kTileM * 128) + row * 128 +
-                                       ((((col >> 2) & 7) ^ (row & 7)) << 4));
-    };
     while (ok && walk->done < walk->todo) {
       int from, to, lim;
       {
+        // What an item needs outside the softmax loop is derived from these copies, which the
+        // compiler cannot see through: what it could hoist out of the walk would sit in the loop's
+        // registers (a row of S takes 128 of 168) and push others into memory, 20% of its time.
+        int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        asm volatile("" : "+r"(lane), "+r"(warp));
+        const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
         const Item it = item_now();
         const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done);
         tile_range(it, t, j0, j0 + seg, from, to);
@@ -653,23 +815,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (m_used == -INFINITY) l = 0.f;
 
       // ------------------------------------------------------------ results of the share
+      int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+      asm volatile("" : "+r"(lane), "+r"(warp));
+      const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+      const uint32_t lane_off = (uint32_t)(quad * 32) << 16, s_tmem = tmem + lane_off + t * kBlockN;
       const Item it = item_now();
       const int j0 = walk->j0, seg = min(it.units - j0, walk->todo - walk->done), item = walk->item;
       Line ln;
       ln.q = walk->line.q, ln.more = walk->line.more, ln.nc = walk->line.nc;
       const int item0 = walk->unit - j0;
       const int me = walk->c, cf = ln.block_of(item0), cl = ln.block_of(item0 + it.units - 1);
-      // A whole item is written at once; a part of one is left as a share in the workspace.
-      const bool direct = !w.prefix_pass && cf == cl;
+      // A whole item is written at once.  A part of one is left as a share in the workspace, and
+      // the warp that leaves the last share of its rows (and columns; each warp has a counter of
+      // its own, nobody waits for anybody) joins them, in block order.  The later of only two
+      // adds the other's share to the O that it has: that sum is the same either way round.
+      const bool split = !w.prefix_pass && cf != cl, two = cl - cf == 1;
+      int* counter = p.counters + cf * 8 + warp;
+      bool all_in = false;
+      if (split && two) {
+        int arrived = 0;
+        if (lane == 0) arrived = ld_acquire_gpu(counter);
+        all_in = __shfl_sync(~0u, arrived, 0) != 0;
+        __threadfence();
+      }
+      const bool leave = w.prefix_pass || (split && !all_in);
       const int row_begin = tile_rows_begin(it, step == 2 ? 0 : t);
       const int quad_rows = max(0, min(32, w.rows - row_begin - quad * 32));  // queries among this warp's rows
       auto slot_of = [&](int x) {
         return w.prefix_pass ? prefix_slot<D>(p.pre, p.Hk, walk->line_id, item, x)
                              : p.partial + (int64_t)(2 * x + (x == cf ? 1 : 0)) * kSlotFloats<D>;
       };
-      // Columns [c0, c1) of O are this warp's to hand on.  With two halves the tiles' warps read
-      // both O_0 and O_1 (the same TMEM lanes) and take half of the columns each.
-      const int c0 = step == 2 ? t * (D / 2) : 0, c1 = step == 2 ? c0 + D / 2 : D;
+      // With two halves the tiles' warps read both O_0 and O_1 (the same TMEM lanes).
       float m_row = m_used, l_row = l, w0 = 1.f, w1 = 0.f;
       bool any0 = t == 0 && any, any1 = t == 1 && any;
       if (step == 2) {
@@ -694,123 +870,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         w0 = w1 = m_used == -INFINITY ? 0.f : 1.f;
       }
-      const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);
-      const float scale = direct && !p.row_share ? inv : 1.f;
-      w0 *= scale, w1 *= scale;
-      float* share = direct ? nullptr : slot_of(me);
+      HandOn<D> h;
+      h.w = &w, h.it = it, h.sQ = sQ, h.tmem = tmem;
+      h.m_row = m_row, h.l_row = l_row, h.w0 = w0, h.w1 = w1, h.any0 = any0, h.any1 = any1;
+      h.row_begin = row_begin, h.quad_rows = quad_rows;
+      h.cf = cf, h.cl = cl, h.me = me;
       if (quad_rows > 0) {
-        if (c0 == 0 && lane < quad_rows) {
-          if (!direct) {
-            *reinterpret_cast<float2*>(share + kWideRows * D + 2 * (t * kTileM + r)) = make_float2(m_row, l_row);
-          } else if (p.row_share) {
-            const Row at = query_row(w, it, row_begin + r);
-            *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * D +
-                                       2 * (int64_t)((at.b * p.n + at.i) * p.H + at.head)) = make_float2(m_row, l_row);
-          } else if (p.lse) {
-            const Row at = query_row(w, it, row_begin + r);
-            p.lse[((int64_t)at.b * p.n + at.i) * p.H + at.head] = l_row == 0.f ? -INFINITY : (m_row + log2f(l_row)) * kLn2;
-          }
-        }
+        bool result = !leave;
 #pragma unroll 1
-        for (int cb = c0; cb < c1; cb += D / 2) {
-#pragma unroll 1
-          for (int x = 0; x < D / 64; ++x) {
-            uint32_t ov[32];
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-            if (any0) {
-              tmem_ld32(tmem + lane_off + C::kOCol + cb + x * 32, ov);
-              tmem_wait_ld();
-              if (w0 != 0.f) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = w0 * __uint_as_float(ov[i]);
-              }
+        for (bool again = true; again;) {
+          hand_on<D, kBf16>(h, result ? nullptr : slot_of(me), lane, warp);
+          again = false;
+          if (!split) break;
+          if (result) {
+            if (lane == 0) *counter = 0;
+          } else {
+            int last = 0;
+            if (lane == 0) {
+              __threadfence();
+              last = atomicAdd(counter, 1) == cl - cf;
             }
-            __syncwarp();
-            if (any1) {
-              tmem_ld32(tmem + lane_off + C::kOCol + D + cb + x * 32, ov);
-              tmem_wait_ld();
-              if (w1 != 0.f) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] += w1 * __uint_as_float(ov[i]);
-              }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            // All shares are there now: join them (of two, the other's, O being still here).
+            result = again = __shfl_sync(~0u, last, 0) != 0;
+            if (again) __threadfence();
           }
-          __syncwarp();
-          if (direct && p.row_share) {  // 4 values a lane, whole rows of D / 2 values
-            constexpr int kLanes = D / 8;
-            const int col = lane % kLanes * 4;
-#pragma unroll 2
-            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes) {
-              const Row at = query_row(w, it, row_begin + quad * 32 + rr);
-              *reinterpret_cast<float4*>(p.row_share + (int64_t)((at.b * p.n + at.i) * p.H + at.head) * D + cb + col) =
-                  *stage_at(quad * 32 + rr, col);
-            }
-          } else if (!direct) {
-            constexpr int kLanes = D / 8;
-            const int col = lane % kLanes * 4;
-            float* dst = share + (step == 2 ? 0 : t * kTileM) * D + cb + col;
-#pragma unroll 4
-            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes)
-              *reinterpret_cast<float4*>(dst + (quad * 32 + rr) * D) = *stage_at(quad * 32 + rr, col);
-          } else {  // 8 values a lane
-            constexpr int kLanes = D / 16;
-            const int col = lane % kLanes * 8;
-#pragma unroll 2
-            for (int rr = lane / kLanes; rr < quad_rows; rr += 32 / kLanes) {
-              const Row at = query_row(w, it, row_begin + quad * 32 + rr);
-              const float4 a = *stage_at(quad * 32 + rr, col), b = *stage_at(quad * 32 + rr, col + 4);
-              if (cb + col < p.D)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh + cb +
-                                          col) =
-                    make_uint4(pack2<kBf16>(a.x, a.y), pack2<kBf16>(a.z, a.w), pack2<kBf16>(b.x, b.y), pack2<kBf16>(b.z, b.w));
-            }
-          }
-          __syncwarp();
         }
       }
       // O_t has been read: the next item's first PV_t may overwrite it once p_half says so.  With
       // two halves the other tile's warps read it too, and Q_0 is shared.
       tc_fence_before();
-      if (step == 2 || (!direct && !w.prefix_pass))
+      if (step == 2)
         if (!(ok = meet())) break;
-      if (!direct && !w.prefix_pass) {
-        // The last block to leave its share of the item joins them all.
-        if (threadIdx.x == 0) {
-          __threadfence();
-          *s_last = atomicAdd(&p.counters[cf], 1) == cl - cf;
-        }
-        if (!(ok = meet())) break;
-        if (*s_last) {
-          __threadfence();
-          constexpr int kLanes = D / 4;  // 4 values a lane
-          const int col = lane % kLanes * 4;
-          const int item_begin = tile_rows_begin(it, 0), item_rows = min(step == 2 ? kTileM : 2 * kTileM, w.rows - item_begin);
-#pragma unroll 1
-          for (int tile_row = warp * (32 / kLanes) + lane / kLanes; tile_row < item_rows; tile_row += 8 * (32 / kLanes)) {
-            const Row at = query_row(w, it, item_begin + tile_row);
-            float mm = -INFINITY, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-            join_shares<D, 4, 4>(
-                cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kWideRows, tile_row, col, mm, ll, v);
-            if (p.row_share) {
-              leave_row<D, 4>(p, (at.b * p.n + at.i) * p.H + at.head, col, mm, ll, v);
-              continue;
-            }
-            const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-            if (col < p.D)
-              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at.b * p.o_sb + at.i * p.o_ss + at.head * p.o_sh + col) =
-                  make_uint2(pack2<kBf16>(v[0] * inv, v[1] * inv), pack2<kBf16>(v[2] * inv, v[3] * inv));
-            if (col == 0 && p.lse)
-              p.lse[((int64_t)at.b * p.n + at.i) * p.H + at.head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
-          }
-          if (threadIdx.x == 0) p.counters[cf] = 0;
-        }
-        if (!(ok = meet())) break;  // s_last is read before the next item writes it
-      }
       // Past this item's share.
       Item nx = it;
       const bool more = walk->done + seg < walk->todo;
