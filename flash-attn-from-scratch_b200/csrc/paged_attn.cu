@@ -404,8 +404,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
     at.advance(p, tiles);
   }
   cp_wait<0>();
-  // The join of the prefix's shares waits for this kernel, and so for the prefix pass before it.
-  if (p.row_share) griddep_wait();
+  // The join of the prefix's shares waits for this kernel, and by its first block for the prefix pass
+  // before it.  (If all blocks waited they would hold the SMs that the others are to run on.)
+  if (p.row_share && blockIdx.x == 0) griddep_wait();
 }
 
 // One warp for each query row: its sums over its own keys and the prefix's shares of it, to `out`.
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const Params p) {
   *reinterpret_cast<V*>(v) = __ldcg(reinterpret_cast<const V*>(p.row_share + (int64_t)row * DP + col));
   const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row));
   float m1[1] = {ml.x}, l1[1] = {ml.y};
-  join_prefix<DP, kPer, 8>(p.pre, p.Hk, hk, b * p.rows + i * p.G + head - hk * p.G, col, m1, l1, v1);
+  join_prefix<DP, kPer, 8>(p.pre, __ldcg(p.counters + kPrefixBlocks), p.Hk, hk, b * p.rows + i * p.G + head - hk * p.G, col, m1, l1, v1);
   const float mm = m1[0], ll = l1[0];
   const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
   if (col < p.D) {
@@ -461,7 +462,7 @@ int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
   constexpr int64_t kUnit = kTeam * kGroup, kTeams = kWarps / kTeam;
   const int64_t most = items * (keys > kUnit ? (keys + kUnit - 1) / kUnit : 1);
   if (grid * kTeams > most) grid = (most + kTeams - 1) / kTeams;
-  if (grid * kTeams > kCounters) grid = kCounters / kTeams;
+  if (grid * kTeams > kPrefixBlocks) grid = kPrefixBlocks / kTeams;
   return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.row_share != nullptr, s, p);
 }
 
@@ -489,9 +490,6 @@ PrefixShares prefix_shares(int64_t rows, int64_t H_kv, int64_t prefix) {
   const int64_t items = s.lines > 1 ? H_kv : H_kv * s.pairs;
   s.nc = sms / s.lines;
   if (s.nc > items * s.units) s.nc = (int)(items * s.units);
-  // As few blocks as leave the longest share as it is: the SMs that are free run the sequences' own keys.
-  const int64_t longest = (items * s.units + s.nc - 1) / s.nc;
-  s.nc = (int)((items * s.units + longest - 1) / longest);
   return s;
 }
 int64_t prefix_floats(const PrefixShares& s, int64_t H_kv, int64_t DP) {

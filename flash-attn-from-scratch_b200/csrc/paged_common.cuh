@@ -57,6 +57,7 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
+constexpr int kPrefixBlocks = 4095;  // of the counters: the count of blocks of a line that the prefix pass used
 constexpr int kCounters = 4096;  // ints at the workspace's start: one per team or warp, zero between calls
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -67,7 +68,7 @@ constexpr float kLn2 = 0.69314718055994531f;
 // all items form one line.
 struct PrefixShares {
   float* slots;  // nullptr: no prefix pass
-  int pairs, units, lines, nc;  // nc: blocks of a line
+  int pairs, units, lines, nc;  // nc: blocks of a line, at most (the pass may leave SMs to the sequences' own keys)
   int tile;      // query rows of a pair: 256, or 128 where there are no more
 };
 constexpr int kWideRows = 256;
@@ -258,14 +259,15 @@ __device__ __forceinline__ void leave_row(const Params& p, int row, int d, float
   if (d == 0) *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row) = make_float2(mm, ll);
 }
 
-// Adds the prefix's shares for query row `row` (of all the batch's rows of K/V head hk).
+// Adds the prefix's shares, of nc blocks a line, for query row `row` (of all the batch's rows of K/V
+// head hk).
 template <int DP, int kPer, int kBatch>
-__device__ __forceinline__ void join_prefix(const PrefixShares& s, int Hk, int hk, int row, int d, float (&mm)[1], float (&ll)[1],
+__device__ __forceinline__ void join_prefix(const PrefixShares& s, int nc, int Hk, int hk, int row, int d, float (&mm)[1], float (&ll)[1],
                                             float (&v)[1][kPer]) {
   const int pair = s.tile == kWideRows ? row / kWideRows : row / (kWideRows / 2), r[1] = {row - pair * s.tile};
   const int line = s.lines > 1 ? pair : 0, item = s.lines > 1 ? hk : hk * s.pairs + pair;
   Line l;
-  l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), s.nc);
+  l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), nc);
   const int cf = l.block_of(item * s.units), cl = l.block_of((item + 1) * s.units - 1);
   join_shares<DP, kPer, 1, kBatch>(
       cl - cf + 1, [&](int x) { return prefix_slot<DP>(s, Hk, line, item, cf + x); }, kWideRows, r, 0, d, mm, ll, v);

@@ -40,6 +40,9 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTileM = 128;
 constexpr int kBlockN = 128;  // keys of a unit
+constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
+constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
+constexpr int kYieldUnits = 8;                       // of a block, up to which the prefix pass yields
 constexpr int kLeast = 4;     // units that a block's share has at least, where there are as many
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 
@@ -73,6 +76,7 @@ struct WideParams {
   int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
   int box_rows;    // rows of a page in one TMA box
   int lines;       // prefix pass: lines of units (paged_common.cuh)
+  int yields;      // prefix pass: may leave SMs to the kernel over the sequences' own keys
 };
 
 // An item's share of a block: blocks [j0, j1) of 128 keys of item (b, hk, pair).
@@ -263,20 +267,20 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
       for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
     __syncwarp();
-    constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes;  // 4 columns a lane
+    constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes, kG = 16 / kRowsPer;  // 4 columns a lane
     const int col = lane % kLanes * 4, sub = lane / kLanes;
 #pragma unroll 1
     for (int x = 0; x < others; ++x) {
       const float f = weight(other_ml(x).x, mm) * inv;
       const float* src = other(x) + (int64_t)o_row * D + cb + col;
 #pragma unroll 1
-      for (int r0 = 0; r0 < quad_rows; r0 += 8 * kRowsPer) {  // eight loads in flight
-        float4 g[8];
+      for (int r0 = 0; r0 < quad_rows; r0 += kG * kRowsPer) {  // 16 rows in flight
+        float4 g[kG];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < kG; ++k)
           g[k] = __ldcg(reinterpret_cast<const float4*>(src + min(r0 + k * kRowsPer + sub, quad_rows - 1) * D));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kG; ++k) {
           const int rr = r0 + k * kRowsPer + sub;
           const float fr = __shfl_sync(~0u, f, rr & 31);
           if (rr >= quad_rows || fr == 0.f) continue;  // a share without a key may not hold O
@@ -362,7 +366,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     first.keys = p.prefix;
     first.visible = p.prefix;
     first.units = p.pre.units;
-    line.cut(first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs), p.pre.nc);
+    const int line_units = first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs);
+    int nc = p.pre.nc;
+    if (w.yields && line_units <= kYieldUnits * nc) {
+      // This pass is bound by the tensor pipe, the one over the sequences' own keys by memory and by
+      // the latency of its start and end, and it may start as soon as SMs are free (it is a
+      // programmatic dependent): the SMs are shared out by the two passes' work, measured by what an
+      // SM does of each in a nanosecond.
+      long long own = 0;
+      for (int b = threadIdx.x; b < p.B; b += kThreads) own += own_length(p, b);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(~0u, own, o);
+      if (lane == 0) scratch[warp] = own;
+      __syncthreads();
+      own = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) own += scratch[i];
+      const float mine = (float)line_units * w.lines * (w.halves == 2 ? kHalfUnitNs : kUnitNs);
+      const float its = (float)own * p.Hk * p.D * (4.f / kSmBytesPerNs);
+      nc = max((nc + 1) / 2, min(nc, (int)(nc * (mine / (mine + its)) + 0.5f)));
+    }
+    // No more blocks than the longest share needs.
+    const int longest = (line_units + nc - 1) / nc;
+    nc = (line_units + longest - 1) / longest;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.counters[kPrefixBlocks] = nc;
+    if (c >= nc) return;
+    line.cut(line_units, nc);
     const int u = line.begin(c), item = (int)((unsigned)u / (unsigned)first.units);
     j_first = u - item * first.units;
     first.b = 0;
@@ -921,8 +950,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, 512);
-  // The join of the prefix's shares waits for this kernel, and so for the prefix pass before it.
-  if (!w.prefix_pass && p.row_share) griddep_wait();
+  // The join of the prefix's shares waits for this kernel, and by its first block for the prefix pass
+  // before it.
+  if (!w.prefix_pass && p.row_share && blockIdx.x == 0) griddep_wait();
 }
 
 template <int D, bool kBf16>
@@ -967,6 +997,7 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   w.pairs = (int)((w.rows + tile - 1) / tile);
   w.box_rows = wide_box_rows(p.page_size);
   w.lines = 1;
+  w.yields = prefix_pass && p.rows <= 16;
   int64_t grid = sm_count();
   if (prefix_pass) {
     w.lines = p.pre.lines;
