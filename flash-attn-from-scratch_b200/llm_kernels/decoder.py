@@ -15,6 +15,10 @@ This is the composition the reference's notebook builds from its modules
 benchmark's decoder-layer workload; there is no residual, activation or down projection.
 Activations never take an extra copy between ops: attention reads q/k/v out of the QKV
 output through strides and writes its output in the layout the O projection reads.
+
+``forward_cached`` is the same layer as it is served: the new tokens' keys go into a paged cache
+(rotated by their positions on the way, the queries with them), and attention reads the cache,
+behind a prefix that the whole batch shares where there is one.
 """
 
 from __future__ import annotations
@@ -24,6 +28,7 @@ import torch.nn as nn
 
 from .flash_attn import flash_attn_forward
 from .int8_gemm import int8_gemm_dequant_nk, int8_gemm_dequant_requant, quantize_symmetric
+from .paged import paged_attention, paged_kv_append, shared_prefix_attention
 
 __all__ = ["DecoderLayerOps"]
 
@@ -62,6 +67,34 @@ class DecoderLayerOps(nn.Module):
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))  # [B, H, T, Dh] views
         attn = torch.empty(B, T, H, Dh, dtype=x.dtype, device=x.device)
         flash_attn_forward(q, k, v, causal=True, out=attn.transpose(1, 2))
+        return self._project(qkv, attn, return_intermediates)
+
+    def forward_cached(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                       block_table: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *,
+                       sections=None, interleaved: bool = False, prefix_pages: torch.Tensor | None = None,
+                       prefix_length: int = 0, return_intermediates: bool = False):
+        """x [B, T, d_model], each sequence's T newest tokens -> [B, T, d_ff].
+
+        k_cache, v_cache [num_pages, page_size, n_heads, head_dim] get the tokens' keys and values in
+        ``slots`` [B * T] (see :func:`cache_slots`); lengths [B] count the keys of each sequence, these
+        tokens' among them; positions [B, T] (or [axes, B, T] with ``sections``) and ``cos_sin`` are
+        those of :func:`rotary_embed`.  With ``prefix_pages`` the sequences follow a shared prefix of
+        ``prefix_length`` keys, which block_table and lengths do not count."""
+        B, T, d = x.shape
+        H, Dh = self.n_heads, self.head_dim
+        qkv = self.qkv(x.reshape(B * T, d)).view(B * T, 3, H, Dh)
+        q = paged_kv_append(qkv[:, 1], qkv[:, 2], k_cache, v_cache, slots, q=qkv[:, 0],
+                            positions=positions.flatten(-2), cos_sin=cos_sin, sections=sections, interleaved=interleaved)
+        q = q.view(B, T, H, Dh)
+        if prefix_pages is None:
+            attn = paged_attention(q, k_cache, v_cache, block_table, lengths)
+        else:
+            attn = shared_prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_length, block_table, lengths)
+        return self._project(qkv.view(B, T, 3, H, Dh), attn, return_intermediates)
+
+    def _project(self, qkv, attn, return_intermediates):
+        B, T = attn.shape[:2]
+        d = self.d_model
         a_q, a_s = quantize_symmetric(attn.view(B * T, d))
         res = int8_gemm_dequant_requant(a_q, self.o_proj.w_q, a_s, self.o_proj.scale_w, "nk",
                                         return_output=return_intermediates)
