@@ -376,24 +376,29 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
       }
       if (last) {
         __threadfence();
-        // A team of four warps has as many rows in flight as one warp alone, in fewer steps.
-        constexpr int kR = kTeam == 1 ? 4 : 1, kBatch = kTeam == 1 ? 3 : 8;
+        // Rows in flight at a time: four of a warp alone; one or two of each warp of a team, as there are.
+        auto join_rows = [&](auto at_once) {
+          constexpr int kR = decltype(at_once)::value, kBatch = kR == 4 ? 3 : 8;
 #pragma unroll 1
-        for (int row0 = in_team * kR; row0 < rows_here; row0 += kTeam * kR) {
-          int r[kR];
-          float mm[kR], ll[kR], v[kR][kPer];
+          for (int row0 = in_team * kR; row0 < rows_here; row0 += kTeam * kR) {
+            int r[kR];
+            float mm[kR], ll[kR], v[kR][kPer];
 #pragma unroll
-          for (int k = 0; k < kR; ++k) {
-            r[k] = min(row0 + k, rows_here - 1);
-            mm[k] = -INFINITY, ll[k] = 0.f;
+            for (int k = 0; k < kR; ++k) {
+              r[k] = min(row0 + k, rows_here - 1);
+              mm[k] = -INFINITY, ll[k] = 0.f;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+              for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+            }
+            join_shares<DP, kPer, kR, kBatch>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, r, 0, col, mm, ll, v);
+#pragma unroll
+            for (int k = 0; k < kR; ++k)
+              if (row0 + k < rows_here) write_out(row0 + k, mm[k], ll[k], v[k]);
           }
-          join_shares<DP, kPer, kR, kBatch>(cl - cf + 1, [&](int x) { return slot_of(cf + x); }, kRows, r, 0, col, mm, ll, v);
-#pragma unroll
-          for (int k = 0; k < kR; ++k)
-            if (row0 + k < rows_here) write_out(row0 + k, mm[k], ll[k], v[k]);
-        }
+        };
+        if constexpr (kTeam == 1) join_rows(std::integral_constant<int, 4>());
+        else if (rows_here > kTeam) join_rows(std::integral_constant<int, 2>());
+        else join_rows(std::integral_constant<int, 1>());
         if (lane == 0 && in_team == 0) p.counters[cf] = 0;
       }
     }
