@@ -78,11 +78,7 @@ void check(const char* name, int status) {
 }
 
 void* stream_on(const Tensor& t) {
-  thread_local int bound = -1;
-  if (bound != t.device.device_id) {
-    check("lk_set_device", lk_set_device(t.device.device_id));
-    bound = t.device.device_id;
-  }
+  check("lk_set_device", lk_set_device(t.device.device_id));  // the library remembers a thread's device
   void* s = nullptr;
   if (g_api->current_work_stream(kDLCUDA, t.device.device_id, &s)) throw Fail{};
   return s;
@@ -241,7 +237,7 @@ void check_caches(const Tensor& k, const Tensor& v, const Tensor& like) {
   require(same, "k_cache and v_cache must be [num_pages, page_size, H_kv, D], of one shape");
   require(k.same_type(like) && v.same_type(like), "the caches must have the dtype of the tokens");
   require(k.flat(3) && v.flat(3), "the caches' last dim must be contiguous");
-  require(k.size(1) > 0, "page_size must be positive");
+  require(k.size(0) > 0 && k.size(1) > 0, "the caches must have a page, and a page a row");
 }
 
 // append(k, v, k_cache, v_cache, slots, q, positions, cos_sin, sections, interleaved, q_out) -> q'

@@ -33,10 +33,18 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;              // query rows of an item
 constexpr int kGroup = 16;             // keys of one warp's step
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
-// Units of 64 prefix keys, over all sequences and K/V heads, from which the prefix pass pays.
-constexpr int64_t kPrefixPass = 1024;
-// Items from which a team is one warp.
+// Units of 64 prefix keys, over all sequences and K/V heads, above which the prefix pass pays; below,
+// each sequence reads the prefix itself, mostly from L2, in one kernel.  (32/8 heads, D = 128, 16
+// sequences: 1024 keys, 2048 units, 20.6 us either way; 256 keys 14.7 against 20.5, 4096 keys 45
+// against 25.)
+constexpr int64_t kPrefixPass = 2048;
+// Items from which a team is one warp.  (64 sequences of 200-8192 keys, 8 K/V heads: 190 us against
+// 211 with teams of four; one sequence of 1000 keys: 20 against 7.5.)
 constexpr int64_t kManyItems = 256;
+// Two tiles of 16 rows read their keys twice, but this kernel starts and joins faster than the one
+// of 256 rows: up to so many keys times K/V heads they take this one.  (32 rows: 8 heads of 8000 keys
+// 29 us against 52, 64 of 2000 35 against 43, 64 of 8000 102 against 78, 512 of 2000 189 against 154.)
+constexpr int64_t kTwoTileKeys = 1 << 18;
 
 template <int DP>
 struct Cfg {
@@ -118,8 +126,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const int per_seq = p.Hk * tiles;
   const int c = blockIdx.x * kTeams + warp / kTeam;  // this warp's team
   Line line;
-  if (!locate<kThreads, kTeams>(p.B, gridDim.x * kTeams, 1, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
-                                [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; }))
+  if (!locate<kThreads, kTeams>(
+          p.B, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
+          [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; },
+          [&](int) { return (int)gridDim.x * kTeams; }))
     return;
   if (c >= line.nc) return;
   Place<kUnit> at;
@@ -582,7 +592,8 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   }
   const int64_t keys = p.prefix + table_cols * page_size;  // of a sequence, at most
   int st;
-  if (p.rows > paged::kRows && wide && p.prefix == 0)
+  const bool few = p.rows <= 2 * paged::kRows && B * H_kv * keys <= paged::kTwoTileKeys;
+  if (p.rows > paged::kRows && wide && p.prefix == 0 && !few)
     st = paged::launch_wide(p, bf16, false, B * H_kv * ((p.rows + 127) / 128) * (keys > 128 ? (keys + 127) / 128 : 1), s);
   else if (D > 64)
     st = bf16 ? paged::launch_rows16<128, true>(p, keys, s) : paged::launch_rows16<128, false>(p, keys, s);

@@ -136,13 +136,11 @@ struct Line {
 
 // Finds where a block's teams (kTeams of them, consecutive on the line from team `team0`) begin, by
 // the whole block: units_of(b) is sequence b's count of units in 64 bits.  Two passes over the lengths: their
-// sum, by which the line is cut into `teams` (fewer, where that leaves them under `least` units: a
-// share costs its join), and a scan up to the places looked for.  found[i] =
+// sum, by which the line is cut among most(sum) teams, and a scan up to the places looked for.  found[i] =
 // (sequence, unit among the sequence's) for team i.  Returns false (reported) if the line does not
 // fit 31 bits, which takes 2^37 keys.  scratch: 8-byte aligned, kThreads / 32 values.
-template <int kThreads, int kTeams, class UnitsOf>
-__device__ __forceinline__ bool locate(int B, int teams, int least, int team0, long long* scratch, int2* found, Line& line,
-                                       UnitsOf units_of) {
+template <int kThreads, int kTeams, class UnitsOf, class Most>
+__device__ __forceinline__ bool locate(int B, int team0, long long* scratch, int2* found, Line& line, UnitsOf units_of, Most most) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long head = (int)threadIdx.x < B ? units_of((int)threadIdx.x) : 0;
@@ -159,7 +157,7 @@ __device__ __forceinline__ bool locate(int B, int teams, int least, int team0, l
     record_bad_index(kSiteLength);
     return false;
   }
-  line.cut((int)all, min(teams, max(1, (int)all / least)));
+  line.cut((int)all, max(1, most((int)all)));
   const int last = line.begin(min(team0 + kTeams, line.nc) - 1);  // the last place looked for
   int base = 0;
   for (int b0 = 0; b0 < B && base <= last; b0 += kThreads) {

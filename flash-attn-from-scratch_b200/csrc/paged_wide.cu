@@ -43,7 +43,7 @@ constexpr int kBlockN = 128;  // keys of a unit
 constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
 constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
 constexpr int kYieldUnits = 8;                       // of a block, up to which the prefix pass yields
-constexpr int kLeast = 4;     // units that a block's share has at least, where there are as many
+constexpr float kJoinUnits = 1.f;  // what the join of a share costs, in units
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 
 enum WideSite : int {
@@ -218,7 +218,6 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
   }
   const float inv = share || p.row_share ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
   const float own = !with_own ? 0.f : others ? weight(h.m_row, mm) * inv : inv;
-  const float f0 = h.w0 == 0.f ? 0.f : h.w0 * own, f1 = h.w1 == 0.f ? 0.f : h.w1 * own;
   uint64_t to = 0;  // where this thread's row goes
   if (lane < quad_rows) {
     if (share) {
@@ -248,23 +247,25 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
       if (h.any0) {
         tmem_ld32(o_tmem + cb + x * 32, ov);
         tmem_wait_ld();
-        if (f0 != 0.f) {
+        if (h.w0 != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = f0 * __uint_as_float(ov[i]);
+          for (int i = 0; i < 32; ++i) v[i] = h.w0 * __uint_as_float(ov[i]);
         }
       }
       __syncwarp();
       if (h.any1) {
         tmem_ld32(o_tmem + D + cb + x * 32, ov);
         tmem_wait_ld();
-        if (f1 != 0.f) {
+        if (h.w1 != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += f1 * __uint_as_float(ov[i]);
+          for (int i = 0; i < 32; ++i) v[i] += h.w1 * __uint_as_float(ov[i]);
         }
       }
       __syncwarp();
+      // The weight goes to the sum, which is what another block would find in the share.
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) *stage_at(r, x * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int i = 0; i < 32; i += 4)
+        *stage_at(r, x * 32 + i) = make_float4(own * v[i], own * v[i + 1], own * v[i + 2], own * v[i + 3]);
     }
     __syncwarp();
     constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes, kG = 16 / kRowsPer;  // 4 columns a lane
@@ -411,7 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int x = 0; x < w.pairs; ++x) sum += units_of_keys(visible_keys(w, L, x));
       return sum;
     };
-    if (!locate<kThreads, 1>(p.B, gridDim.x, kLeast, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; }))
+    // A share costs about a unit's time when it is joined, and the shares of an item are joined one
+    // after the other: units / nc + nc / items is least at this nc.  (One sequence of 8 x 32 rows:
+    // 2000 keys 29 us, against 37 where a join counts two units or four.)
+    const float items = (float)p.B * p.Hk * w.pairs;
+    if (!locate<kThreads, 1>(
+            p.B, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; },
+            [&](int units) { return min((int)gridDim.x, (int)(sqrtf(units * items * (1.f / kJoinUnits)) + 1.f)); }))
       return;
     if (c >= line.nc) return;
     first.b = found->x;

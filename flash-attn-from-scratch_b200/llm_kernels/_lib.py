@@ -196,14 +196,9 @@ def i64_array(vals) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
 
 
-_tls = threading.local()
-
-
 def set_device(index: int) -> None:
-    """Makes device ``index`` current for the library on this thread (cached)."""
-    if getattr(_tls, "device", None) != index:
-        call("lk_set_device", int(index))
-        _tls.device = index
+    """Makes device ``index`` current for the library on this thread (which remembers it)."""
+    call("lk_set_device", int(index))
 
 
 def device_status() -> tuple[int, int, int, int]:

@@ -292,6 +292,38 @@ def test_streams_and_graphs():
     cases[0].check(out[0])
 
 
+@pytest.mark.parametrize("B,n,prefix", [(40, 1, 3000), (70, 1, 9000), (6, 30, 5000)])
+def test_prefix_pass_on_streams_and_in_a_graph(B, n, prefix):
+    """The kernels of a long prefix, which overlap: beside another stream's, captured, replayed with
+    other lengths, and called again at once."""
+    cases = [Case([(17 * b + s) % 300 for b in range(B)], n=n, prefix=prefix, seed=s, H=8, Hk=2) for s in (0, 1)]
+    want = [c.call(return_lse=True) for c in cases]
+    for c, (o, lse) in zip(cases, want):
+        c.check(o, lse)
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(c.call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i][0]) for i in (0, 1) for o in got[i])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [c.call() for c in cases]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w[0]) for o, w in zip(out, want))
+    cases[0].lengths_list = [max(0, L - 40) for L in cases[0].lengths_list]
+    cases[0].lengths.copy_(torch.tensor(cases[0].lengths_list, dtype=torch.int32))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    cases[0].check(out[0])
+    assert torch.equal(out[0], cases[0].call())
+
+
 def test_slots_and_append_then_attend():
     """Tokens appended one by one and in pieces give what a whole cache gives."""
     g = torch.Generator("cuda").manual_seed(3)
@@ -341,6 +373,8 @@ def test_refusals():
     ):
         with pytest.raises(E):
             bad()
+    with pytest.raises(E):
+        P(c.q, c.k[:0], c.v[:0], c.table, c.lengths)
     big = torch.zeros(1, 1, 2, 136, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(E):
         P(big, big, big, c.table[:1], c.lengths[:1])
