@@ -188,8 +188,8 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
   const bool halves = w.halves == 2, two = h.cl - h.cf == 1;
   const int quad_rows = h.quad_rows, c0 = halves ? t * (D / 2) : 0, c1 = halves ? c0 + D / 2 : D;
   const uint32_t o_tmem = h.tmem + ((uint32_t)(quad * 32) << 16) + C::kOCol;
-  // Row r of the tile, columns 4 .. of 32 in 32 bits, in this warp's own rows of the tile's Q buffer
-  // (128-byte swizzle).
+  // Row `row` of the tile, columns col .. col + 3 of the D / 2 at hand in 32 bits, in this warp's own
+  // rows of the tile's Q buffer (128-byte swizzle).
   auto stage_at = [&](int row, int col) {
     return reinterpret_cast<float4*>(h.sQ + t * C::kTile + (col >> 5) * (kTileM * 128) + row * 128 +
                                      ((((col >> 2) & 7) ^ (row & 7)) << 4));
@@ -218,6 +218,8 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
   }
   const float inv = share || p.row_share ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
   const float own = !with_own ? 0.f : others ? weight(h.m_row, mm) * inv : inv;
+  // No weight, no value: where the shares are all read from the workspace, O counts there.
+  const float w0 = own == 0.f ? 0.f : h.w0, w1 = own == 0.f ? 0.f : h.w1;
   uint64_t to = 0;  // where this thread's row goes
   if (lane < quad_rows) {
     if (share) {
@@ -247,18 +249,18 @@ __device__ __forceinline__ void hand_on(const HandOn<D>& h, float* share, int la
       if (h.any0) {
         tmem_ld32(o_tmem + cb + x * 32, ov);
         tmem_wait_ld();
-        if (h.w0 != 0.f) {
+        if (w0 != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = h.w0 * __uint_as_float(ov[i]);
+          for (int i = 0; i < 32; ++i) v[i] = w0 * __uint_as_float(ov[i]);
         }
       }
       __syncwarp();
       if (h.any1) {
         tmem_ld32(o_tmem + D + cb + x * 32, ov);
         tmem_wait_ld();
-        if (h.w1 != 0.f) {
+        if (w1 != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += h.w1 * __uint_as_float(ov[i]);
+          for (int i = 0; i < 32; ++i) v[i] += w1 * __uint_as_float(ov[i]);
         }
       }
       __syncwarp();
@@ -801,14 +803,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < kBlockN / 2; ++e) {
           const uint64_t x2 = fma2(f2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, ng2);
-          float x0, x1, p0, p1;
+          float x0, x1;
           uf2(x2, x0, x1);
-          if ((e & 7) == 0) {
-            fa::exp2_poly_pair(x0, x1, p0, p1);
-          } else {
-            p0 = fa::ex2(x0);
-            p1 = fa::ex2(x1);
-          }
+          const float p0 = fa::ex2(x0), p1 = fa::ex2(x1);
           rs2 = add2(rs2, f2(p0, p1));
           pk[e] = pack2<kBf16>(p0, p1);  // rounded for the matrix product; the sum is of the unrounded
           if (e == kBlockN / 4 - 1) {
@@ -845,10 +842,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 2;
         tc_fence_after();
       }
-      // A row that saw no key has m = -inf (its l is of the 2^-125 that the polynomial gives for
-      // a masked key); one whose scores were not numbers keeps that.
+      // A row that saw no key has m = -inf, l = 0; one whose scores were not numbers stays so.
       if (l != l) m_used = fmaxf(m_used, 0.f);
-      if (m_used == -INFINITY) l = 0.f;
 
       // ------------------------------------------------------------ results of the share
       int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

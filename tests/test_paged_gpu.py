@@ -201,6 +201,25 @@ def test_infinite_values(n):
     c.check(out, lse)
 
 
+@pytest.mark.parametrize("n,L,prefix", [(1, 20000, 0), (4, 300, 0), (40, 2500, 0), (8, 2500, 0), (20, 40000, 0), (1, 30, 5000), (300, 700, 0)])
+def test_values_that_are_not_finite(n, L, prefix):
+    """An infinite value stays one in its column, a key that is no number makes its head's rows so, and
+    nothing else changes -- whichever blocks and shares they pass through."""
+    c = Case([L, L // 2], n=n, H=8, Hk=2, prefix=prefix, dtype=torch.bfloat16, scale=0.3)
+    clean = c.call()
+    at = c.prefix_pages if prefix else c.table[0]
+    c.v[at[0].long(), 5, 0, 17] = math.inf
+    c.k[at[0].long(), 7, 1, 3] = math.nan
+    out, lse = c.call(return_lse=True)
+    hit = out if prefix else out[:1]
+    assert (hit[:, :, :4, 17] == math.inf).all()
+    assert hit[:, :, 4:].isnan().all() and (lse if prefix else lse[:1])[:, :, 4:].isnan().all()
+    rest = torch.arange(128, device="cuda") != 17
+    assert torch.equal(hit[:, :, :4][..., rest], (clean if prefix else clean[:1])[:, :, :4][..., rest])
+    if not prefix:
+        assert torch.equal(out[1], clean[1])
+
+
 def test_offsets_past_32_bits():
     """Pages whose offsets pass 2^31 values and 2^32 bytes."""
     page, Hk, D = 64, 8, 128
