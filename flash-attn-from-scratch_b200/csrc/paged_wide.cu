@@ -23,6 +23,12 @@
 // serial chain; there tile 1 takes the same queries over every second key block (two halves of
 // the keys, joined at the item's end: the two tiles' warps see the same lanes of tensor memory).
 //
+// Measured (B200, 32/8 heads, D = 128, bf16): 2.2 us for a unit of 256 rows x 128 keys, as the
+// flash-attention forward takes (1100 TFLOP/s); 4 x 500 prompt tokens at up to 9000 keys 222 us (720
+// TFLOP/s: a share costs 15-20 thousand cycles besides its units, for Q, the first S, and the way of O
+// through memory where blocks share an item).  A launch of one unit takes 12 us, mostly instruction
+// fetches and round trips to memory that nothing hides yet.
+//
 // Keys behind a sequence's last one: whole boxes of them are not read (an out-of-range page
 // coordinate gives zeros); in the box that holds the end the rows of V behind it are zeroed in
 // shared memory before the MMA may see them (0 x NaN), and S is masked.

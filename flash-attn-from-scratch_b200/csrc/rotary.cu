@@ -8,7 +8,9 @@
 // The map is a rotation, so its gradient is the rotation by -s (inverse).
 //
 // Bound: memory.  A token's heads are read and written once and nothing is reused but the table
-// rows (8 bytes a pair, from L1 / L2).
+// rows (8 bytes a pair, from L1 / L2).  Measured (B200, bf16, D = 128): 16380 tokens of 32/8 heads
+// with three axes and their gradient 112 us, 6.2 TB/s; append of 16384 tokens of 32 heads 132 us,
+// 6.2 TB/s (a copy runs at 6.5).  16 tokens: 3.5 us, two round trips to memory and the launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

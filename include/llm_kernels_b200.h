@@ -375,14 +375,19 @@ LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const v
  *   strides:   12 element strides: (b, n, h) of q and out, (page, row, h) of k_cache and v_cache,
  *              multiples of 8 with 16-byte aligned bases; the d strides are 1.
  *   D:         a multiple of 8 up to 128.  dtype LK_F16 or LK_BF16.  softmax_scale <= 0 = D^-0.5.
- *   workspace: lk_paged_attention_workspace_bytes(...) bytes, 256-byte aligned, zeroed once
- *              before its first use; every call leaves its counters at zero again, so calls on
- *              one stream share it and calls that can overlap do not.
+ *   workspace: lk_paged_attention_workspace_bytes(...) bytes (prefix_length 0 for
+ *              lk_paged_attention; a larger one serves too), 256-byte aligned, zeroed once before
+ *              its first use; every call leaves its counters at zero again, so calls on one
+ *              stream share it and calls that can overlap do not.  After a device failure (a
+ *              wait that ran out) zero it again.
+ * Results do not depend on timing: the same call gives the same bits.
  *
  * lk_shared_prefix_attention: the same for a batch whose sequences share their first
  * prefix_length keys, held in the pages prefix_pages[0 ..]; every token sees all of them, and
- * they are read and multiplied once for the whole batch.  block_table and lengths name what
- * follows the prefix, from the start of a page of its own; lengths[b] may be 0. */
+ * they are read and multiplied once for the whole batch (where the batch and the prefix are small
+ * each sequence reads them itself, in one kernel; otherwise up to three kernels run, the later
+ * ones as programmatic dependents).  block_table and lengths name what follows the prefix, from
+ * the start of a page of its own; lengths[b] may be 0. */
 LK_API int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D,
                                                   int64_t prefix_length);
 LK_API int lk_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
