@@ -134,7 +134,16 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   if (!locate<kThreads, kTeams>(
           p.B, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
           [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; },
-          [&](int) { return (int)gridDim.x * kTeams; }))
+          [&](int units) {
+            // Beside a prefix pass that yields: as many blocks as run at once on the SMs it leaves (a
+            // second wave of them would begin when it ends), unless this pass is much the longer one.
+            const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
+            if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
+            const float bytes = (float)units * kUnit * p.D * 4.f;
+            const int kept = yielding_blocks(p.pre, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
+            return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
+                                                                                           : (int)gridDim.x * kTeams;
+          }))
     return;
   if (c >= line.nc) return;
   Place<kUnit> at;
@@ -577,6 +586,7 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   p.B = (int)B, p.n = (int)n, p.H = (int)H, p.Hk = (int)H_kv, p.G = (int)(H / H_kv), p.D = (int)D;
   p.rows = p.n * p.G;
   p.by_G = paged::FastDiv::of(p.G), p.by_rows = paged::FastDiv::of(p.rows), p.by_page = paged::FastDiv::of(page_size);
+  p.sms = sm_count();
   p.num_pages = (int)num_pages, p.page_size = (int)page_size, p.prefix = (int)prefix_length;
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = scale * 1.4426950408889634f;

@@ -90,6 +90,7 @@ struct Params {
   int num_pages, page_size, table_cols;
   FastDiv by_G, by_rows, by_page;                    // of G, rows and page_size
   int prefix;                                        // keys before the sequences' own, common to all
+  int sms;
   float scale_log2;
   int* counters;   // [kCounters]
   float* partial;  // slots of partial sums
@@ -117,6 +118,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // exp2 of a difference of two log2-scaled maxima, 0 where the first is -inf (also beside -inf).
 __device__ __forceinline__ float weight(float m, float top) { return m == -INFINITY ? 0.f : fa::ex2(m - top); }
+
+// The prefix pass is bound by the tensor pipe, the one over the sequences' own keys by memory and by
+// the latency of its start and end, and that one may start as soon as SMs are free (it is a
+// programmatic dependent).  A short prefix pass therefore yields: the SMs are shared out by the two
+// passes' work, measured by what an SM does of each in a nanosecond.  (32 sequences of 1-512 keys
+// behind 8192: 53 us without.  Over 8 units a block the passes slow each other more than the overlap
+// gives: 256 sequences behind 32768 keys 282 us against 267.)
+constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
+constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
+constexpr float kStartNs = 12000.f;                      // a launch of the pass, before and behind its units
+constexpr int kYieldUnits = 8;                           // of a block, up to which the prefix pass yields
+__device__ __forceinline__ bool yields(const PrefixShares& s, int line_units) { return line_units <= kYieldUnits * s.nc; }
+// What the pass takes on nc blocks a line.
+__device__ __forceinline__ float prefix_ns(const PrefixShares& s, int line_units, int nc) {
+  return kStartNs + (float)((line_units + nc - 1) / nc) * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs);
+}
+// Blocks of a line that the prefix pass keeps beside `bytes` of the sequences' own keys.
+__device__ __forceinline__ int yielding_blocks(const PrefixShares& s, int line_units, float bytes) {
+  const float mine = (float)line_units * s.lines * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs), its = bytes / kSmBytesPerNs;
+  return max((s.nc + 1) / 2, min(s.nc, (int)(s.nc * (mine / (mine + its)) + 0.5f)));
+}
 
 // The line of units of a launch and its even cut: the first `more` blocks have q + 1 units, the
 // others q.

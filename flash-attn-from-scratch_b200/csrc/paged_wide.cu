@@ -46,9 +46,6 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTileM = 128;
 constexpr int kBlockN = 128;  // keys of a unit
-constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
-constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
-constexpr int kYieldUnits = 8;                       // of a block, up to which the prefix pass yields
 constexpr float kJoinUnits = 1.f;  // what the join of a share costs, in units
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 
@@ -377,11 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     first.units = p.pre.units;
     const int line_units = first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs);
     int nc = p.pre.nc;
-    if (w.yields && line_units <= kYieldUnits * nc) {
-      // This pass is bound by the tensor pipe, the one over the sequences' own keys by memory and by
-      // the latency of its start and end, and it may start as soon as SMs are free (it is a
-      // programmatic dependent): the SMs are shared out by the two passes' work, measured by what an
-      // SM does of each in a nanosecond.
+    if (w.yields && yields(p.pre, line_units)) {
       long long own = 0;
       for (int b = threadIdx.x; b < p.B; b += kThreads) own += own_length(p, b);
 #pragma unroll
@@ -391,9 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       own = 0;
 #pragma unroll
       for (int i = 0; i < kThreads / 32; ++i) own += scratch[i];
-      const float mine = (float)line_units * w.lines * (w.halves == 2 ? kHalfUnitNs : kUnitNs);
-      const float its = (float)own * p.Hk * p.D * (4.f / kSmBytesPerNs);
-      nc = max((nc + 1) / 2, min(nc, (int)(nc * (mine / (mine + its)) + 0.5f)));
+      nc = yielding_blocks(p.pre, line_units, (float)own * p.Hk * p.D * 4.f);
     }
     // No more blocks than the longest share needs.
     const int longest = (line_units + nc - 1) / nc;
