@@ -220,6 +220,20 @@ def test_values_that_are_not_finite(n, L, prefix):
         assert torch.equal(out[1], clean[1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_whole_prompt_is_causal_flash_attention(dtype):
+    """All of a prompt's tokens as its newest ones: the flash-attention forward's result, whose
+    roundings are the same kind (its exponentials are good to 2^-13)."""
+    c = Case([1500, 1500], n=1500, H=8, Hk=2, dtype=dtype, poison=False)
+    got = c.call()
+    k, v = (torch.stack([c.rows(x, c.table[b], 1500) for b in (0, 1)]).to(dtype).transpose(1, 2) for x in (c.k, c.v))
+    other = llm_kernels.flash_attn_forward(c.q.transpose(1, 2), k, v, causal=True).transpose(1, 2)
+    want, _, size, far = c.exact()
+    u = UNIT[dtype]
+    tol = 2 * (u * want.abs() + (u + 2.0 ** -12) * size + (2.0 ** -25 * far if u < 2.0 ** -10 else 0.0))
+    assert ((got.double() - other.double()).abs() <= tol).all()
+
+
 def test_offsets_past_32_bits():
     """Pages whose offsets pass 2^31 values and 2^32 bytes."""
     page, Hk, D = 64, 8, 128
