@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
             // second wave of them would begin when it ends), unless this pass is much the longer one.
             const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
             if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
-            const float bytes = (float)units * kUnit * p.D * 4.f;
-            const int kept = yielding_blocks(p.pre, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
+            const float bytes = fmaxf((float)units * kUnit, (float)p.B * per_seq * kLeastKeys) * p.D * 4.f;
+            const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
             return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
                                                                                            : (int)gridDim.x * kTeams;
           }))

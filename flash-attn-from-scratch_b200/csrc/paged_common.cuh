@@ -57,7 +57,8 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
-constexpr int kPrefixBlocks = 4095;  // of the counters: the count of blocks of a line that the prefix pass used
+// Of the counters: the count of blocks of a line that the prefix pass used, or minus that of an item.
+constexpr int kPrefixBlocks = 4095;
 constexpr int kCounters = 4096;  // ints at the workspace's start: one per team or warp, zero between calls
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -128,6 +129,7 @@ __device__ __forceinline__ float weight(float m, float top) { return m == -INFIN
 constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
 constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
 constexpr float kStartNs = 12000.f;                      // a launch of the pass, before and behind its units
+constexpr int kLeastKeys = 64;                           // that a sequence's own keys count for at least
 constexpr int kYieldUnits = 8;                           // of a block, up to which the prefix pass yields
 __device__ __forceinline__ bool yields(const PrefixShares& s, int line_units) { return line_units <= kYieldUnits * s.nc; }
 // What the pass takes on nc blocks a line.
@@ -135,9 +137,9 @@ __device__ __forceinline__ float prefix_ns(const PrefixShares& s, int line_units
   return kStartNs + (float)((line_units + nc - 1) / nc) * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs);
 }
 // Blocks of a line that the prefix pass keeps beside `bytes` of the sequences' own keys.
-__device__ __forceinline__ int yielding_blocks(const PrefixShares& s, int line_units, float bytes) {
+__device__ __forceinline__ int yielding_blocks(const PrefixShares& s, int sms, int line_units, float bytes) {
   const float mine = (float)line_units * s.lines * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs), its = bytes / kSmBytesPerNs;
-  return max((s.nc + 1) / 2, min(s.nc, (int)(s.nc * (mine / (mine + its)) + 0.5f)));
+  return max((s.nc + 1) / 2, min(s.nc, (int)(sms / s.lines * (mine / (mine + its)) + 0.5f)));
 }
 
 // The line of units of a launch and its even cut: the first `more` blocks have q + 1 units, the
@@ -214,6 +216,24 @@ __device__ __forceinline__ bool locate(int B, int team0, long long* scratch, int
   return true;
 }
 
+__device__ __forceinline__ int up_div(int a, int b) { return (int)((unsigned)(a + b - 1) / (unsigned)b); }
+
+// Blocks of each item of the prefix pass if its items are cut one by one (nc becomes their count), 0 if
+// their line is cut evenly among nc blocks.  A share costs about as much as kShareUnits units besides its
+// own (Q, the first S, and the way of O through memory), and in the even cut most blocks have the end of
+// one item and the begin of the next.  (32/8 heads: 16 sequences without own keys behind 16384 37 us against
+// 47, 128 of 1-20 keys behind 3000 33 against 49.  A long prefix pass beside single tokens keeps the even
+// cut, which leaves a few SMs more to them: 32 sequences behind 20000 keys 56 us against 58.)
+constexpr int kShareUnits = 1;
+__device__ __forceinline__ int blocks_per_item(int items, int units, int& nc) {
+  if (items == 1 || items > nc) return 0;
+  const int part = up_div(units, (int)((unsigned)nc / (unsigned)items));
+  if (part > up_div(units * items, nc) + kShareUnits) return 0;
+  const int used = up_div(units, part);
+  nc = used * items;
+  return used;
+}
+
 template <int DP>
 __device__ __forceinline__ float* prefix_slot(const PrefixShares& s, int Hk, int line, int item, int block) {
   // (item, block) pairs walk a staircase, so item + block numbers them.
@@ -279,16 +299,21 @@ __device__ __forceinline__ void leave_row(const Params& p, int row, int d, float
   if (d == 0) *reinterpret_cast<float2*>(p.row_share + (int64_t)p.B * p.n * p.H * DP + 2 * (int64_t)row) = make_float2(mm, ll);
 }
 
-// Adds the prefix's shares, of nc blocks a line, for query row `row` (of all the batch's rows of K/V
-// head hk).
+// Adds the prefix's shares, of nc blocks a line (negative: of -nc blocks an item), for query row `row`
+// (of all the batch's rows of K/V head hk).
 template <int DP, int kPer, int kBatch>
 __device__ __forceinline__ void join_prefix(const PrefixShares& s, int nc, int Hk, int hk, int row, int d, float (&mm)[1], float (&ll)[1],
                                             float (&v)[1][kPer]) {
   const int pair = s.tile == kWideRows ? row / kWideRows : row / (kWideRows / 2), r[1] = {row - pair * s.tile};
   const int line = s.lines > 1 ? pair : 0, item = s.lines > 1 ? hk : hk * s.pairs + pair;
   Line l;
-  l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), nc);
-  const int cf = l.block_of(item * s.units), cl = l.block_of((item + 1) * s.units - 1);
+  int cf, cl;
+  if (nc < 0) {
+    cf = item * -nc, cl = cf - nc - 1;
+  } else {
+    l.cut(s.units * (s.lines > 1 ? Hk : Hk * s.pairs), nc);
+    cf = l.block_of(item * s.units), cl = l.block_of((item + 1) * s.units - 1);
+  }
   join_shares<DP, kPer, 1, kBatch>(
       cl - cf + 1, [&](int x) { return prefix_slot<DP>(s, Hk, line, item, cf + x); }, kWideRows, r, 0, d, mm, ll, v);
 }

@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Line line;
   Item first;
   int c, line_id = 0;
-  int j_first;
+  int j_first, u0, todo;
   if (w.prefix_pass) {
     c = blockIdx.x;
     if (w.lines > 1) {
@@ -372,11 +372,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     first.keys = p.prefix;
     first.visible = p.prefix;
     first.units = p.pre.units;
-    const int line_units = first.units * p.Hk * (w.lines > 1 ? 1 : w.pairs);
+    const int items = p.Hk * (w.lines > 1 ? 1 : w.pairs), line_units = first.units * items;
     int nc = p.pre.nc;
-    if (w.yields && yields(p.pre, line_units)) {
+    const bool brief = yields(p.pre, line_units);
+    if (w.yields && brief) {
       long long own = 0;
-      for (int b = threadIdx.x; b < p.B; b += kThreads) own += own_length(p, b);
+      for (int b = threadIdx.x; b < p.B; b += kThreads) own += max(own_length(p, b), kLeastKeys);
 #pragma unroll
       for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(~0u, own, o);
       if (lane == 0) scratch[warp] = own;
@@ -384,16 +385,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       own = 0;
 #pragma unroll
       for (int i = 0; i < kThreads / 32; ++i) own += scratch[i];
-      nc = yielding_blocks(p.pre, line_units, (float)own * p.Hk * p.D * 4.f);
+      nc = yielding_blocks(p.pre, p.sms, line_units, (float)own * p.Hk * p.D * 4.f);
     }
-    // No more blocks than the longest share needs.
-    const int longest = (line_units + nc - 1) / nc;
-    nc = (line_units + longest - 1) / longest;
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.counters[kPrefixBlocks] = nc;
+    const int per_item = (brief || !w.yields) ? blocks_per_item(items, first.units, nc) : 0;
+    if (!per_item) {  // no more blocks than the longest share needs
+      const int longest = up_div(line_units, nc);
+      nc = up_div(line_units, longest);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.counters[kPrefixBlocks] = per_item ? -per_item : nc;
     if (c >= nc) return;
-    line.cut(line_units, nc);
-    const int u = line.begin(c), item = (int)((unsigned)u / (unsigned)first.units);
-    j_first = u - item * first.units;
+    int item;
+    if (per_item) {
+      line.cut(first.units, per_item);
+      item = (int)((unsigned)c / (unsigned)per_item);
+      j_first = line.begin(c - item * per_item);
+      u0 = item * first.units + j_first;
+      todo = line.begin(c - item * per_item + 1) - j_first;
+    } else {
+      line.cut(line_units, nc);
+      u0 = line.begin(c), todo = line.begin(c + 1) - u0;
+      item = (int)((unsigned)u0 / (unsigned)first.units);
+      j_first = u0 - item * first.units;
+    }
     first.b = 0;
     first.hk = item;
     first.pair = line_id;
@@ -432,10 +445,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++first.pair;
       enter(w, first);
     }
+    u0 = line.begin(c), todo = line.begin(c + 1) - u0;
     __syncthreads();  // the scratch is Q's
   }
-  const int u0 = line.begin(c);
-  const int todo = line.begin(c + 1) - u0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
