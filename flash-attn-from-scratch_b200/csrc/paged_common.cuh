@@ -124,7 +124,7 @@ __device__ __forceinline__ float weight(float m, float top) { return m == -INFIN
 // the latency of its start and end, and that one may start as soon as SMs are free (it is a
 // programmatic dependent).  A short prefix pass therefore yields: the SMs are shared out by the two
 // passes' work, measured by what an SM does of each in a nanosecond.  (32 sequences of 1-512 keys
-// behind 8192: 53 us without.  Over 8 units a block the passes slow each other more than the overlap
+// behind 8192: 36 us, 53 without.  Over 8 units a block the passes slow each other more than the overlap
 // gives: 256 sequences behind 32768 keys 282 us against 267.)
 constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
 constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all

@@ -425,8 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       return sum;
     };
     // A share costs about a unit's time when it is joined, and the shares of an item are joined one
-    // after the other: units / nc + nc / items is least at this nc.  (One sequence of 8 x 32 rows:
-    // 2000 keys 29 us, against 37 where a join counts two units or four.)
+    // after the other: units / nc + nc / items is least at this nc.  (64 tokens of 32/8
+    // heads at 2000 keys: 43 us, against 53 where a join counts two units and 55 where it counts a half.)
     const float items = (float)p.B * p.Hk * w.pairs;
     if (!locate<kThreads, 1>(
             p.B, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; },
