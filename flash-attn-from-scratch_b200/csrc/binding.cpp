@@ -23,7 +23,7 @@ const DLPackExchangeAPI* g_api = nullptr;
 PyObject* g_tensor = nullptr;     // torch.Tensor
 PyObject* g_empty_like = nullptr;
 PyObject* g_new_lse = nullptr;    // (q, shape) -> fp32 tensor
-PyObject* g_capturing = nullptr;  // () -> bool
+PyObject* g_capturing = nullptr;  // (device index) -> bool: of the current stream there
 PyObject* g_zeros = nullptr;      // (device index, bytes) -> uint8 tensor
 PyObject* g_input_error = nullptr;
 PyObject* g_call_error = nullptr;  // (name, status, detail) -> exception
@@ -78,7 +78,7 @@ void check(const char* name, int status) {
 }
 
 void* stream_on(const Tensor& t) {
-  check("lk_set_device", lk_set_device(t.device.device_id));  // the library remembers a thread's device
+  check("lk_set_device", lk_set_device(t.device.device_id));  // for the default stream, which names none
   void* s = nullptr;
   if (g_api->current_work_stream(kDLCUDA, t.device.device_id, &s)) throw Fail{};
   return s;
@@ -386,10 +386,15 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (B > 0 && n > 0 && H > 0) {
       void* stream = stream_on(q);
       const int64_t need = lk_paged_attention_workspace_bytes(B, n, H, Hk, D, prefix);
-      Ref capturing(PyObject_CallNoArgs(g_capturing));
+      bool capturing = false;
+      if (stream) {  // the legacy default stream cannot be captured
+        Ref device(PyLong_FromLong(q.device.device_id));
+        Ref yes(PyObject_CallOneArg(g_capturing, device.o));
+        capturing = yes.o == Py_True;
+      }
       Workspace ws{};
       PyObject* own = nullptr;
-      if (capturing.o == Py_True) {
+      if (capturing) {
         // A graph may be replayed beside this stream's other work: it keeps a workspace of its own.
         own = PyObject_CallFunction(g_zeros, "iL", (int)q.device.device_id, (long long)need);
         if (!own) throw Fail{};

@@ -557,7 +557,8 @@ int forward(const void* q, const void* k, const void* v, void* o, float* lse, in
   const int64_t nqb = (M + 2 * fa::kTileM - 1) / (2 * fa::kTileM);
   if (nqb * B * H > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   const bool bf16 = dtype == LK_BF16;
   CUtensorMap tq, tk, tv;
   if (int st = fa::make_map(&tq, bf16, q, B, H, M, D, q_strides)) return st;

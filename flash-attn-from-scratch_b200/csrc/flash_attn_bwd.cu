@@ -765,7 +765,8 @@ extern "C" int lk_flash_attn_bwd(const void* q, const void* k, const void* v, co
       if (vec_st[i][j] % 8) return LK_ERR_ALIGNMENT;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   const bool bf16 = dtype == LK_BF16;
   CUtensorMap tq, tk, tv, tdo;
   if (int st = fa::make_map(&tq, bf16, q, B, H, M, D, sq)) return st;

@@ -67,7 +67,8 @@ int run_int8(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, int b_l
     if (!aligned16(dsts[d])) return LK_ERR_ALIGNMENT;
   // Multicast stores are whole 16-byte vectors of whole 32-column chunks.
   if (multimem && (num_dst != 1 || N % 32)) return LK_ERR_ALIGNMENT;
-  if (int st = bind_stream(stream)) return st;
+  const DeviceScope scope(stream);
+  if (scope.status()) return scope.status();
   auto set_scatter = [&](gemm::Params& p) {
     p.num_dst = num_dst;
     p.dst_multimem = multimem;
@@ -182,7 +183,8 @@ int run_int8_requant(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb,
   if (lda < K || ldq < N || (C && ldc < N)) return LK_ERR_INVALID_ARG;
   if (b_mn ? (ldb < N) : (ldb < K)) return LK_ERR_INVALID_ARG;
   if (lda % 16 || ldb % 16 || ldq % 16 || !aligned16(q)) return LK_ERR_ALIGNMENT;
-  if (int st = bind_stream(stream)) return st;
+  const DeviceScope scope(stream);
+  if (scope.status()) return scope.status();
   const int num_sms = sm_count();
   const int ptm = (int)((M + 255) / 256), ptn = (int)((N + 255) / 256);
   // Every tile of a row block must sit on its own pair, and every pair of the grid must be

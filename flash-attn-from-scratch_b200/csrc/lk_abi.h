@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "../../include/llm_kernels_b200.h"
+#include "device_scope.h"
 
 namespace lk {
 
@@ -16,15 +17,32 @@ int cuda_status(cudaError_t err);
 // cudaGetLastError() after a launch, mapped to a status.
 inline int check_launch() { return cuda_status(cudaGetLastError()); }
 
-// Makes `dev` current in this library's runtime on the calling thread, with its primary
-// context (cached per thread).
-int bind_device(int dev);
+// The CUDA calls of DeviceSwitch (device_scope.h).
+struct CudaApi {
+  static int current_device(int* dev);
+  static int current_context(void** ctx);
+  static int set_context(void* ctx);
+  static int set_device(int dev);
+};
 
-// Binds to the stream's device (for the NULL stream: to the device set with lk_set_device, or
-// device 0).
-int bind_stream(cudaStream_t stream);
+// For the length of a call, makes current the device (with its primary context, which driver calls
+// such as TMA descriptor encoding need) that the call runs on, and then the caller's again.
+class DeviceScope {
+ public:
+  // The stream's device; for the NULL stream the one that lk_set_device picked (or an earlier call
+  // bound), or device 0.
+  explicit DeviceScope(cudaStream_t stream);
+  explicit DeviceScope(int device);
+  // For calls that name no stream: ThreadDevice::for_status.
+  DeviceScope();
+  int status() const { return status_; }  // LK_OK, or LK_ERR_CUDA: nothing may be launched
 
-// Streaming multiprocessor count of the current device (cached per device).
+ private:
+  DeviceSwitch<CudaApi> switch_;
+  int status_;
+};
+
+// Streaming multiprocessor count of the device that this thread's calls run on (cached per device).
 int sm_count();
 
 // Builds a tiled TMA descriptor (row-major tensor, dims/strides innermost first; strides in

@@ -18,11 +18,7 @@ __device__ unsigned long long g_wait_limit_ns = 1000000000ull;
 
 namespace {
 thread_local int t_last_cuda_error = 0;
-// Device this library made current on the calling thread with cudaSetDevice (-1: none yet).
-// cudaGetDevice alone cannot tell: it reports device 0 on a fresh thread without making any
-// context current, and the driver calls of this library (TMA descriptor encoding) need one --
-// e.g. on the worker thread that runs autograd's backward.
-thread_local int t_bound_device = -1;
+thread_local ThreadDevice t_device;
 
 constexpr int kMaxDevices = 64;
 int g_sm_count[kMaxDevices];
@@ -50,29 +46,74 @@ int cuda_status(cudaError_t err) {
   return LK_ERR_CUDA;
 }
 
-int bind_device(int dev) {
-  if (t_bound_device == dev) return LK_OK;
-  const int st = cuda_status(cudaSetDevice(dev));  // makes the device's primary context current
-  if (st == LK_OK) t_bound_device = dev;
+namespace {
+struct ContextCalls {
+  PFN_cuCtxGetDevice_v2000 device = nullptr;
+  PFN_cuCtxGetCurrent_v4000 get = nullptr;
+  PFN_cuCtxSetCurrent_v4000 set = nullptr;
+  ContextCalls() {
+    load("cuCtxGetDevice", device);
+    load("cuCtxGetCurrent", get);
+    load("cuCtxSetCurrent", set);
+  }
+  template <class F>
+  static void load(const char* name, F& f) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint(name, &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      f = reinterpret_cast<F>(fn);
+    else
+      cudaGetLastError();
+  }
+};
+const ContextCalls& context_calls() {
+  static const ContextCalls c;
+  return c;
+}
+}  // namespace
+
+// The driver is asked: the runtime's cudaGetDevice reports device 0 on a thread without a context.
+int CudaApi::current_device(int* dev) {
+  CUdevice d = -1;
+  const auto f = context_calls().device;
+  const int st = f ? (int)f(&d) : (int)CUDA_ERROR_NOT_FOUND;
+  *dev = (int)d;
   return st;
 }
+int CudaApi::current_context(void** ctx) {
+  const auto f = context_calls().get;
+  return f ? (int)f(reinterpret_cast<CUcontext*>(ctx)) : (int)CUDA_ERROR_NOT_FOUND;
+}
+int CudaApi::set_context(void* ctx) {
+  const auto f = context_calls().set;
+  return f ? (int)f(static_cast<CUcontext>(ctx)) : (int)CUDA_ERROR_NOT_FOUND;
+}
+int CudaApi::set_device(int dev) { return cuda_status(cudaSetDevice(dev)); }
 
-int bind_stream(cudaStream_t stream) {
-  if (stream == nullptr) return t_bound_device >= 0 ? LK_OK : bind_device(0);
-  // A capturing stream may not be asked for its device (the query ends the capture with an
-  // error): the device that lk_set_device or an earlier call bound is taken.
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone && t_bound_device >= 0)
-    return LK_OK;
-  int dev = -1;
-  const int st = cuda_status(cudaStreamGetDevice(stream, &dev));
-  if (st != LK_OK) return st;
-  return bind_device(dev);
+DeviceScope::DeviceScope(int device) : status_(switch_.to(device, t_device)) {}
+
+DeviceScope::DeviceScope() : status_(switch_.to(t_device.for_status(DeviceSwitch<CudaApi>::now()), t_device)) {}
+
+DeviceScope::DeviceScope(cudaStream_t stream) {
+  int dev = t_device.for_null_stream();
+  if (stream != nullptr) {
+    // A capturing stream may not be asked for its device (the query ends the capture with an
+    // error): the device that lk_set_device or an earlier call bound is taken, or the current one.
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
+      const int now = DeviceSwitch<CudaApi>::now();
+      if (t_device.device < 0 && now >= 0) dev = now;
+    } else if ((status_ = cuda_status(cudaStreamGetDevice(stream, &dev))) != LK_OK) {
+      return;
+    }
+  }
+  status_ = switch_.to(dev, t_device);
 }
 
 int sm_count() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  int dev = t_device.device;
+  if (dev < 0 && cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 0 || dev >= kMaxDevices) return 148;
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_sm_count[dev] > 0) return g_sm_count[dev];
@@ -207,11 +248,23 @@ int lk_last_cuda_error(void) { return lk::t_last_cuda_error; }
 
 int lk_version(void) { return (1 << 16) | 0; }
 
-int lk_set_device(int device) { return lk::bind_device(device); }
+int lk_set_device(int device) {
+  using namespace lk;
+  if (device < 0 || device != t_device.device) {
+    int n = 0;
+    if (int st = cuda_status(cudaGetDeviceCount(&n))) return st;
+    if (device < 0 || device >= n) return cuda_status(cudaErrorInvalidDevice);
+  }
+  t_device.device = device;
+  t_device.seen = DeviceSwitch<CudaApi>::now();
+  return LK_OK;
+}
 
 int lk_device_status(int* out4) {
   int h[4] = {0, 0, 0, 0};
-  int st = lk::cuda_status(cudaDeviceSynchronize());
+  const lk::DeviceScope scope;
+  int st = scope.status();
+  if (st == LK_OK) st = lk::cuda_status(cudaDeviceSynchronize());
   if (st != LK_OK) return st;
   st = lk::cuda_status(cudaMemcpyFromSymbol(h, lk::g_status, sizeof(h)));
   if (st != LK_OK) return st;
@@ -226,7 +279,9 @@ int lk_device_status(int* out4) {
 
 int lk_debug_set_wait_limit(int64_t ns) {
   const unsigned long long v = ns > 0 ? (unsigned long long)ns : 1000000000ull;
-  int st = lk::cuda_status(cudaDeviceSynchronize());
+  const lk::DeviceScope scope;
+  int st = scope.status();
+  if (st == LK_OK) st = lk::cuda_status(cudaDeviceSynchronize());
   if (st != LK_OK) return st;
   return lk::cuda_status(cudaMemcpyToSymbol(lk::g_wait_limit_ns, &v, sizeof(v)));
 }
@@ -241,7 +296,9 @@ int lk_debug_inject(int kind, int block, int item) {
 
 int lk_clear_device_status(void) {
   int z[4] = {0, 0, 0, 0};
-  int st = lk::cuda_status(cudaDeviceSynchronize());
+  const lk::DeviceScope scope;
+  int st = scope.status();
+  if (st == LK_OK) st = lk::cuda_status(cudaDeviceSynchronize());
   if (st != LK_OK) return st;
   // A split GEMM launch that gave up may have left its tail counters non-zero.
   st = lk::cuda_status((cudaError_t)lk::gemm::reset_split_workspaces());

@@ -571,7 +571,8 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   for (int i = 0; i < 12; ++i)
     if (strides[i] % 8) return LK_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
       workspace_bytes < lk_paged_attention_workspace_bytes(B, n, H, H_kv, D, prefix_length))
     return LK_ERR_INVALID_ARG;

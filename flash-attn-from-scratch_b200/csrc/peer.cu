@@ -53,7 +53,8 @@ PFN_cuMemGetAddressRange_v3020 address_range() {
 extern "C" int lk_peer_export(int device, const void* ptr, void* handle_out, int64_t* offset_out) {
   using namespace lk;
   if (!ptr || !handle_out || !offset_out) return LK_ERR_INVALID_ARG;
-  if (int st = lk_set_device(device)) return st;
+  const DeviceScope scope(device);
+  if (scope.status()) return scope.status();
   auto range = address_range();
   if (!range) return LK_ERR_UNSUPPORTED;
   CUdeviceptr base = 0;
@@ -70,7 +71,8 @@ extern "C" int lk_peer_export(int device, const void* ptr, void* handle_out, int
 extern "C" int lk_peer_open(int device, const void* handle, int64_t offset, void** ptr_out) {
   using namespace lk;
   if (!handle || !ptr_out || offset < 0) return LK_ERR_INVALID_ARG;
-  if (int st = lk_set_device(device)) return st;
+  const DeviceScope scope(device);
+  if (scope.status()) return scope.status();
   HandleKey key;
   key.first = device;
   memcpy(key.second.data(), handle, LK_PEER_HANDLE_BYTES);
@@ -94,7 +96,8 @@ extern "C" int lk_peer_open(int device, const void* handle, int64_t offset, void
 extern "C" int lk_peer_close(int device, void* ptr, int64_t offset) {
   using namespace lk;
   if (!ptr || offset < 0) return LK_ERR_INVALID_ARG;
-  if (int st = lk_set_device(device)) return st;
+  const DeviceScope scope(device);
+  if (scope.status()) return scope.status();
   void* base = static_cast<uint8_t*>(ptr) - offset;
   std::lock_guard<std::mutex> lock(g_map_mu);
   auto bit = g_by_base.find(std::make_pair(device, reinterpret_cast<uintptr_t>(base)));

@@ -341,7 +341,8 @@ extern "C" int lk_quantize_symmetric(const void* x, int x_dtype, int64_t rows, i
   if (x_ld < cols || q_ld < cols) return LK_ERR_INVALID_ARG;
   if (rows > (int64_t)0x7FFFFFFF * kWarpsPerCta) return LK_ERR_INVALID_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   switch (x_dtype) {
     case LK_F32:
       return launch_quantize<float>(x, rows, cols, x_ld, q, q_ld, scale, s);

@@ -293,7 +293,8 @@ extern "C" int lk_rmsnorm_linear_fold(const void* w_norm, int w_norm_dtype, cons
   if (d_in % 8) return LK_ERR_INVALID_ARG;
   if (!aligned16(w_lin) || !aligned16(w_fold)) return LK_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   return dtype == LK_F16 ? run_fold<__half>(w_norm, w_norm_dtype, w_lin, w_fold, d_in, d_out, s)
                          : run_fold<__nv_bfloat16>(w_norm, w_norm_dtype, w_lin, w_fold, d_in, d_out, s);
 }
@@ -310,7 +311,8 @@ int rmsnorm_linear(const void* x, int64_t x_ld, const void* w_fold, void* y, int
   if (rows > INT32_MAX / 2 || d_in > INT32_MAX / 2 || d_out > INT32_MAX / 2) return LK_ERR_INVALID_ARG;
   if (!aligned16(x) || !aligned16(w_fold)) return LK_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   return dtype == LK_F16
              ? run_gemm<gemm::Kind::F16>(x, x_ld, w_fold, y, y_ld, rows, d_in, d_out, eps, row_rstd, s, may_allocate)
              : run_gemm<gemm::Kind::BF16>(x, x_ld, w_fold, y, y_ld, rows, d_in, d_out, eps, row_rstd, s,
@@ -396,9 +398,12 @@ extern "C" int lk_rmsnorm_linear_noalloc(const void* x, int64_t x_ld, const void
   if (rows < 0 || d_in < 0 || d_out < 0) return LK_ERR_INVALID_ARG;
   if (rows > kStaticRstdRows) return LK_ERR_SCRATCH_LIMIT;
   if (rows == 0 || d_out == 0) return LK_OK;
-  if (int st = bind_stream(static_cast<cudaStream_t>(stream))) return st;
   float* rstd = nullptr;
-  if (int st = static_rstd_address(&rstd)) return st;
+  {
+    const DeviceScope scope(static_cast<cudaStream_t>(stream));
+    if (scope.status()) return scope.status();
+    if (int st = static_rstd_address(&rstd)) return st;
+  }
   // Every element of rstd[0, rows) is written by the row kernel before the GEMM reads it, so
   // whatever the previous call left in the array needs no clearing.
   return rmsnorm_linear(x, x_ld, w_fold, y, y_ld, dtype, rows, d_in, d_out, eps, rstd, stream, false);

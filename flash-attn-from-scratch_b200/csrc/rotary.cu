@@ -423,7 +423,8 @@ extern "C" int lk_rotary_embed(const void* q, void* q_out, const void* k, void* 
                                interleaved))
     return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   return rot::launch<false>(p, dtype == LK_BF16, B * S, s);
 }
 
@@ -472,6 +473,7 @@ extern "C" int lk_paged_kv_append(const void* q, void* q_out, const void* k, con
                                  interleaved))
       return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int st = bind_stream(s)) return st;
+  const DeviceScope scope(s);
+  if (scope.status()) return scope.status();
   return rot::launch<true>(p, dtype == LK_BF16, T, s);
 }

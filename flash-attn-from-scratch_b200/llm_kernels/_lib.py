@@ -144,6 +144,16 @@ def load() -> ctypes.CDLL:
 _binding = None
 
 
+def _capturing(device: int) -> bool:
+    """Whether torch's current stream on ``device``, which need not be the current one, is being captured."""
+    import torch
+
+    if device == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _call_error(name: str, status: int, cuda: int) -> LKError:
     return LKError(name, status, f"cudaError {cuda}" if cuda else "")
 
@@ -165,7 +175,7 @@ def binding():
                 torch.Tensor,
                 torch.empty_like,
                 lambda q: torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device),
-                torch.cuda.is_current_stream_capturing,
+                _capturing,
                 lambda dev, n: torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda", dev)),
                 LKInputError,
                 _call_error,
@@ -197,14 +207,15 @@ def i64_array(vals) -> ctypes.Array:
 
 
 def set_device(index: int) -> None:
-    """Makes device ``index`` current for the library on this thread (which remembers it)."""
+    """Picks the device of this thread's calls on the default stream; torch's current device stays."""
     call("lk_set_device", int(index))
 
 
 def device_status() -> tuple[int, int, int, int]:
     """Synchronises and returns the device status word (code, site, block, thread): code 4 for a
     pipeline wait that ran out, 1 for an index out of range in device data (a cache slot, a page
-    id, a position, a length)."""
+    id, a position, a length).  The device is that of this thread's last call, or torch's current
+    one if that has been changed since."""
     out = (ctypes.c_int * 4)()
     st = load().lk_device_status(out)
     if st not in (LK_OK, LK_ERR_TIMEOUT, LK_ERR_INVALID_ARG):

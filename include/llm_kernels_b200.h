@@ -57,12 +57,14 @@ LK_API int lk_last_cuda_error(void);
 /* ABI version: (major << 16) | minor. */
 LK_API int lk_version(void);
 
-/* Makes `device` the current device for this library's calls on the calling host thread.
- * Entry points given a non-NULL stream bind to that stream's device themselves; calls on the
- * legacy default stream (NULL) run on the device set here (default 0). */
+/* Picks the device of this library's calls on the calling host thread.  Entry points given a
+ * non-NULL stream run on that stream's device; calls on the legacy default stream (NULL) run on
+ * the device picked here (default 0).  No entry point changes the caller's current device or
+ * context: each switches for its own length where it has to. */
 LK_API int lk_set_device(int device);
 
-/* Synchronises the current device, then copies its status word into out4 (may be NULL):
+/* Synchronises a device -- that of the thread's last call or lk_set_device, or the current one where
+ * the caller has changed it since -- then copies its status word into out4 (may be NULL):
  * out4[0] = lk_status of the first device failure (0 = none), out4[1] = failure site id,
  * out4[2] = blockIdx.x, out4[3] = threadIdx.x of the thread that recorded it.
  * LK_ERR_INVALID_ARG means that a kernel met an index out of range in the caller's device data
@@ -78,8 +80,8 @@ LK_API int lk_device_status(int* out4);
  * and leaves the context usable.  Nothing faults: the hooks only withhold one copy or one
  * counter update, so a consumer's bounded wait ends with an error status. */
 
-/* Limit of every bounded device wait on the current device, in nanoseconds (<= 0 restores the
- * default of one second).  Synchronous. */
+/* Limit of every bounded device wait on lk_device_status's device, in nanoseconds (<= 0 restores
+ * the default of one second).  Synchronous. */
 LK_API int lk_debug_set_wait_limit(int64_t ns);
 
 /* Arms a one-shot injection, taken by the next launch of the named kernel in this process:
@@ -102,7 +104,7 @@ typedef enum {
 } lk_inject;
 LK_API int lk_debug_inject(int kind, int block, int item);
 
-/* Resets the current device's status word to 0 (synchronous), and re-zeroes the counters of
+/* Resets the status word of lk_device_status's device to 0 (synchronous), and re-zeroes the counters of
  * every split workspace of the device, which a launch that gave up may have left non-zero.
  * After a non-zero status, results of launches up to this call are not to be trusted. */
 LK_API int lk_clear_device_status(void);
