@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._common import require
-from .rotary import expand_positions
+from .rotary import expand_positions, has_tangent
 
 __all__ = ["cache_slots", "paged_kv_append", "paged_attention", "shared_prefix_attention"]
 
@@ -56,7 +56,14 @@ def paged_kv_append(k, v, k_cache, v_cache, slots, *, q=None, positions=None, co
 
     Returns:
         the rotated queries, or None without q.
+
+    Not differentiable: q, k or v that a derivative is asked of (grad mode with ``requires_grad``, or a
+    forward-mode tangent) are refused.  Training rotates with :func:`rotary_embed`.
     """
+    grad = torch.is_grad_enabled()
+    for t in (k, v, q):
+        require(not (grad and getattr(t, "requires_grad", False)) and not has_tangent(t),
+                "paged_kv_append has no gradient: call it under torch.no_grad(), or rotate with rotary_embed to train")
     if sections is not None:
         sections = tuple(sections)
     append = _lib.binding().append

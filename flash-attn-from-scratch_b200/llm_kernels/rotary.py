@@ -82,9 +82,9 @@ class RotaryFunction(torch.autograd.Function):
         return rotate(tq, tk, positions, cos_sin, *ctx.how)
 
 
-def _has_tangent(x) -> bool:
+def has_tangent(x) -> bool:
     # Without an open dual level there is none; that is asked first because unpacking costs 0.35 us.
-    return getattr(forward_ad, "_current_level", 0) >= 0 and x is not None and forward_ad.unpack_dual(x).tangent is not None
+    return getattr(forward_ad, "_current_level", 0) >= 0 and isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None
 
 
 def rotary_embed(q, k, positions, cos_sin, *, sections=None, interleaved=False, inverse=False):
@@ -110,7 +110,7 @@ def rotary_embed(q, k, positions, cos_sin, *, sections=None, interleaved=False, 
     require(isinstance(cos_sin, torch.Tensor) and not cos_sin.requires_grad, "cos_sin must be a tensor that needs no gradient")
     if sections is not None:
         sections = tuple(sections)
-    dual = _has_tangent(q), _has_tangent(k)
+    dual = has_tangent(q), has_tangent(k)
     if k is not None and dual[0] != dual[1]:  # the function's outputs all have one, or none
         return tuple(rotary_embed(x, None, positions, cos_sin, sections=sections, interleaved=interleaved, inverse=inverse)
                      for x in (q, k))
