@@ -38,11 +38,15 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;              // query rows of an item
 constexpr int kGroup = 16;             // keys of one warp's step
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
-// Units of 64 prefix keys, over all sequences and K/V heads, above which the prefix pass pays; below,
-// each sequence reads the prefix itself, mostly from L2, in one kernel.  (32/8 heads, D = 128, 16
-// sequences: 1024 keys, 2048 units, 20.6 us either way; 256 keys 14.7 against 20.5, 4096 keys 45
-// against 25.)
-constexpr int64_t kPrefixPass = 2048;
+// Units of 64 prefix keys, over all sequences, K/V heads and tiles of 16 query rows, above which the
+// prefix pass pays; below, each tile reads the prefix itself, mostly from L2, in one kernel.  One tile
+// alone shares nothing.  (32/8 heads, D = 128, one kernel against the pass.  16 single tokens: 256 keys
+// 15 us against 19, 1024 keys, 2048 units, 21 either way, 4096 keys 46 against 23.  20 tokens of each of
+// two sequences: 512 keys, 640 units, 19 either way, 4096 keys 38 against 25.  One piece of 500 tokens:
+// 64 keys 54 against 62, 256 keys, 4000 units, 64 either way, 8192 keys 487 against 124.  Of 252 calls
+// of 1-32 sequences, 1-500 tokens, 64-16384 keys and five head layouts the rule's choice takes 2.7% more
+// than the better one; at 2048 units it is 2.9%, at 6144 4.8%.)
+constexpr int64_t kPrefixPass = 3072;
 // Items from which a team is one warp.  (64 sequences of 200-8192 keys, 8 K/V heads: 190 us against
 // 211 with teams of four; one sequence of 1000 keys: 20 against 7.5.)
 constexpr int64_t kManyItems = 256;
@@ -597,7 +601,9 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   const int64_t DP = D > 64 ? 128 : 64;
   bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
   for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
-  if (prefix_length > 0 && wide && B * H_kv * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
+  const int64_t row_tiles = (p.rows + paged::kRows - 1) / paged::kRows;
+  if (prefix_length > 0 && wide && B * row_tiles > 1 &&
+      B * H_kv * row_tiles * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
     paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
     if ((int64_t)pre.units * H_kv * pre.pairs > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
     pre.slots = p.partial + paged::own_floats(p.rows, DP);

@@ -119,7 +119,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, softmax_scale=
 def shared_prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_length, block_table, lengths, *, softmax_scale=None,
                             out=None, return_lse=False):
     """:func:`paged_attention` for a batch whose sequences share their first ``prefix_length``
-    keys, which are read and multiplied once for all of them.
+    keys, which are read and multiplied once for all of them (each sequence reads them itself where
+    that is little work, or where the page size is no multiple of 8).
 
     Args:
         prefix_pages : [pages] int32, the pages that hold the prefix.

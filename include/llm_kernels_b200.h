@@ -386,9 +386,10 @@ LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const v
  *
  * lk_shared_prefix_attention: the same for a batch whose sequences share their first
  * prefix_length keys, held in the pages prefix_pages[0 ..]; every token sees all of them, and
- * they are read and multiplied once for the whole batch (where the batch and the prefix are small
- * each sequence reads them itself, in one kernel; otherwise up to three kernels run, the later
- * ones as programmatic dependents).  block_table and lengths name what follows the prefix, from
+ * they are read and multiplied once for the whole batch, 256 query rows of a K/V head at a time, by
+ * up to three kernels, the later ones as programmatic dependents.  (Where the prefix's keys times the
+ * batch's tiles of 16 query rows are few, or page_size is no multiple of 8, each tile reads the prefix
+ * itself, in one kernel.)  block_table and lengths name what follows the prefix, from
  * the start of a page of its own; lengths[b] may be 0. */
 LK_API int64_t lk_paged_attention_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t H_kv, int64_t D,
                                                   int64_t prefix_length);
