@@ -4,7 +4,9 @@
 // CUDA in the process), and either may change it between two calls: what this library made current
 // once says nothing about now, so every call asks.  A call that has to switch puts the caller's
 // context back when it ends -- the context, not a device number: to set a device is to create a
-// context on it, and a thread that had none is to have none again.
+// context on it, and a thread that had none is to have none again.  Device 0 is the exception: it is
+// where a thread without a context is anyway, so its context may stay (torch's autograd threads begin
+// so, and warn if they find none).
 //
 // Host code without CUDA in it, so that a test can run it against a stand-in.  Api is that of the
 // driver and runtime; its functions return 0 or an error:
@@ -47,7 +49,7 @@ class DeviceSwitch {
     const int was = now();
     if (was != dev) {
       // A context that is current but answers for no device has been destroyed: not put back.
-      restore_ = Api::current_context(&before_) == 0 && (was >= 0 || before_ == nullptr);
+      restore_ = Api::current_context(&before_) == 0 && (was >= 0 || (before_ == nullptr && dev != 0));
       if (const int st = Api::set_device(dev)) return st;
     }
     t.device = dev;

@@ -59,8 +59,8 @@ LK_API int lk_version(void);
 
 /* Picks the device of this library's calls on the calling host thread.  Entry points given a
  * non-NULL stream run on that stream's device; calls on the legacy default stream (NULL) run on
- * the device picked here (default 0).  No entry point changes the caller's current device or
- * context: each switches for its own length where it has to. */
+ * the device picked here (default 0).  No entry point changes the caller's current device:
+ * each switches for its own length where it has to. */
 LK_API int lk_set_device(int device);
 
 /* Synchronises a device -- that of the thread's last call or lk_set_device, or the current one where

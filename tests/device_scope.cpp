@@ -92,6 +92,8 @@ int main() {
     start(-1);
     CHECK(call(t, 1) == 1 && g_current == nullptr && !g_primary[0].alive);
     CHECK(call(t, 1) == 1 && g_current == nullptr);
+    CHECK(call(t, 0) == 0 && current() == 0);  // but device 0 is where such a thread is
+    CHECK(call(t, 1) == 1 && current() == 0);
   }
   {  // A device that cannot be set: the error, and the caller's context.
     lk::ThreadDevice t;

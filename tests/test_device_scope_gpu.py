@@ -14,34 +14,44 @@ from llm_kernels import _lib
 pytestmark = pytest.mark.gpu
 
 
-def test_a_thread_without_a_context_has_none_afterwards():
-    x = torch.randn(40, 256, device="cuda", dtype=torch.float16)
-    q, s = torch.zeros(40, 256, device="cuda", dtype=torch.int8), torch.zeros(40, device="cuda")
+def test_a_thread_without_a_context():
+    """Its calls run on the device picked, by default device 0, where CUDA has such a thread anyway."""
+    x = torch.randn(40, 256, device="cuda:0", dtype=torch.float16)
+    q, s = torch.zeros(40, 256, device="cuda:0", dtype=torch.int8), torch.zeros(40, device="cuda:0")
     torch.cuda.synchronize()
     cuda, seen = ctypes.CDLL("libcuda.so.1"), []
 
     def current():
-        ctx = ctypes.c_void_p(1)
+        dev, ctx = ctypes.c_int(-1), ctypes.c_void_p(1)
         assert cuda.cuCtxGetCurrent(ctypes.byref(ctx)) == 0
-        return ctx.value
+        return None if ctx.value is None else (cuda.cuCtxGetDevice(ctypes.byref(dev)), dev.value)
 
     def work():
         seen.append(current())
-        for call in (lambda: _lib.call("lk_set_device", 0),
-                     lambda: _lib.call("lk_quantize_symmetric", x.data_ptr(), _lib.LK_F16, 40, 256, 256, q.data_ptr(), 256,
-                                       s.data_ptr(), None),
-                     llm_kernels.device_status):
-            call()
-            seen.append(current())
+        _lib.call("lk_set_device", 0)  # picks, and makes nothing current
+        seen.append(current())
+        _lib.call("lk_quantize_symmetric", x.data_ptr(), _lib.LK_F16, 40, 256, 256, q.data_ptr(), 256, s.data_ptr(), None)
+        seen.append(current())
+        seen.append(llm_kernels.device_status()[0])
+        seen.append(torch.cuda.current_device())
 
     t = threading.Thread(target=work)
     t.start()
     t.join()
     torch.cuda.synchronize()
-    assert seen == [None] * 4
+    assert seen == [None, None, (0, 0), 0, 0]
     want, scale = oracle.quantize_symmetric(x.cpu())
     np.testing.assert_array_equal(q.cpu().numpy(), want)
     np.testing.assert_array_equal(s.cpu().numpy(), scale)
+
+
+def test_backward_on_autograds_thread_finds_a_context(recwarn):
+    """The library's backward is the first CUDA work of torch's autograd thread; a matrix product follows."""
+    q = torch.randn(6, 4, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(64, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = llm_kernels.rotary_embed(q @ w, None, torch.arange(6, device="cuda"), llm_kernels.rotary_table(6, 64))
+    y.backward(torch.ones_like(y))
+    assert w.grad.isfinite().all() and not [r for r in recwarn if "context" in str(r.message)]
 
 
 def test_the_callers_device_stays():
