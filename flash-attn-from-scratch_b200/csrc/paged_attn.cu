@@ -35,8 +35,10 @@ namespace paged {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;              // query rows of an item
 constexpr int kGroup = 16;             // keys of one warp's step
+// log2 of the keys of a team's step, its unit: 16 keys a warp.
+constexpr int team_shift(int team) { return team == 1 ? 4 : 6; }
+static_assert(1 << team_shift(1) == kGroup && 1 << team_shift(kWarps) == kWarps * kGroup, "units of a team's warps");
 constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before O is rescaled
 // Units of 64 prefix keys, over all sequences, K/V heads and tiles of 16 query rows, above which the
 // prefix pass pays; below, each tile reads the prefix itself, mostly from L2, in one kernel.  One tile
@@ -90,15 +92,15 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A place on the line of units: a team's step is kUnit keys.
-template <int kUnit>
+// A place on the line of units: a team's step is 2^kShift keys.
+template <int kShift>
 struct Place {
   int b, hk, rt;  // item: sequence, K/V head, tile of 16 rows
   int j, units;   // unit of the item, and how many it has
   int keys;       // prefix + own keys of the sequence
   __device__ __forceinline__ void enter(const Params& p) {
     keys = b < p.B ? p.prefix + own_length(p, b) : 0;
-    units = max(1, (keys + kUnit - 1) / kUnit);
+    units = units_of(keys, kShift);
   }
   __device__ __forceinline__ void advance(const Params& p, int tiles) {
     if (++j < units) return;
@@ -116,7 +118,7 @@ template <int DP, bool kBf16, int kTeam>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params p) {
   using C = Cfg<DP>;
   constexpr int kStages = C::kStages;
-  constexpr int kUnit = kTeam * kGroup;
+  constexpr int kShift = team_shift(kTeam), kUnit = 1 << kShift;
   constexpr int kTeams = kWarps / kTeam;   // of a block
   constexpr int kChunks = DP / 8;          // 16-byte pieces of a row
   constexpr int kPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
@@ -132,25 +134,25 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int in_team = warp % kTeam;  // this warp's place in its team
   const int tiles = (p.rows + kRows - 1) / kRows;
-  const int per_seq = p.Hk * tiles;
+  const int per_seq = own_items(p);
   const int c = blockIdx.x * kTeams + warp / kTeam;  // this warp's team
   Line line;
   if (!locate<kThreads, kTeams>(
           p.B, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
-          [&](int b) { return (long long)max(1, (p.prefix + own_length(p, b) + kUnit - 1) / kUnit) * per_seq; },
+          [&](int b) { return (long long)units_of(p.prefix + own_length(p, b), kShift) * per_seq; },
           [&](int units) {
             // Beside a prefix pass that yields: as many blocks as run at once on the SMs it leaves (a
             // second wave of them would begin when it ends), unless this pass is much the longer one.
             const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
             if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
-            const float bytes = fmaxf((float)units * kUnit, (float)p.B * per_seq * kLeastKeys) * p.D * 4.f;
+            const float bytes = own_bytes(p, units, per_seq);
             const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
             return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
                                                                                            : (int)gridDim.x * kTeams;
           }))
     return;
   if (c >= line.nc) return;
-  Place<kUnit> at;
+  Place<kShift> at;
   at.b = s_found[warp / kTeam].x;
   at.enter(p);
   const int offset = s_found[warp / kTeam].y;
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * C::kTile);
   const int chunk = lane % kChunks, sub = lane / kChunks;
   const bool chunk_in = chunk * 8 < p.D;
-  Place<kUnit> ld = at;
+  Place<kShift> ld = at;
   int ld_left = todo;
   // Lane l (and l + 16) looks up the page of key l of this warp's step, one step ahead; the entry
   // is not looked at before its turn.
@@ -492,17 +494,22 @@ int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
     configured.fetch_or(bit);
   }
   int64_t grid = 2 * (int64_t)sm_count();
-  constexpr int64_t kUnit = kTeam * kGroup, kTeams = kWarps / kTeam;
+  constexpr int64_t kUnit = 1 << team_shift(kTeam), kTeams = kWarps / kTeam;
   const int64_t most = items * (keys > kUnit ? (keys + kUnit - 1) / kUnit : 1);
   if (grid * kTeams > most) grid = (most + kTeams - 1) / kTeams;
   if (grid * kTeams > kPrefixBlocks) grid = kPrefixBlocks / kTeams;
   return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.row_share != nullptr, s, p);
 }
 
+// Warps of a team.
+int team_of(const Params& p) {
+  return (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows) >= kManyItems ? 1 : kWarps;
+}
+
 template <int DP, bool kBf16>
 int launch_rows16(const Params& p, int64_t keys, cudaStream_t s) {
   const int64_t items = (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows);
-  return items >= kManyItems ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
+  return team_of(p) == 1 ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
 }
 
 }  // namespace paged
@@ -602,20 +609,23 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
   for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
   const int64_t row_tiles = (p.rows + paged::kRows - 1) / paged::kRows;
-  if (prefix_length > 0 && wide && B * row_tiles > 1 &&
-      B * H_kv * row_tiles * ((prefix_length + 63) / 64) > paged::kPrefixPass) {
+  const bool pass = prefix_length > 0 && wide && B * row_tiles > 1 &&
+                    B * H_kv * row_tiles * ((prefix_length + 63) / 64) > paged::kPrefixPass;
+  const int64_t keys = (pass ? 0 : prefix_length) + table_cols * page_size;  // of a sequence, at most
+  const bool few = p.rows <= 2 * paged::kRows && B * H_kv * keys <= paged::kTwoTileKeys;
+  const bool own_wide = p.rows > paged::kRows && wide && (pass || prefix_length == 0) && !few;
+  if (pass) {
     paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
     if ((int64_t)pre.units * H_kv * pre.pairs > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
     pre.slots = p.partial + paged::own_floats(p.rows, DP);
+    pre.own_shift = own_wide ? 0 : paged::team_shift(paged::team_of(p));
     p.pre = pre;
     p.row_share = pre.slots + paged::prefix_floats(pre, H_kv, DP);
     if (int st = paged::launch_wide(p, bf16, true, 0, s)) return st;
     p.prefix = 0;
   }
-  const int64_t keys = p.prefix + table_cols * page_size;  // of a sequence, at most
   int st;
-  const bool few = p.rows <= 2 * paged::kRows && B * H_kv * keys <= paged::kTwoTileKeys;
-  if (p.rows > paged::kRows && wide && p.prefix == 0 && !few)
+  if (own_wide)
     st = paged::launch_wide(p, bf16, false, B * H_kv * ((p.rows + 127) / 128) * (keys > 128 ? (keys + 127) / 128 : 1), s);
   else if (D > 64)
     st = bf16 ? paged::launch_rows16<128, true>(p, keys, s) : paged::launch_rows16<128, false>(p, keys, s);

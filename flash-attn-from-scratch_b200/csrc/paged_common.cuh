@@ -71,6 +71,8 @@ struct PrefixShares {
   float* slots;  // nullptr: no prefix pass
   int pairs, units, lines, nc;  // nc: blocks of a line, at most (the pass may leave SMs to the sequences' own keys)
   int tile;      // query rows of a pair: 256, or 128 where there are no more
+  int own_shift;  // log2 of the keys of a unit of the 16-row kernel, if that one takes the own keys: it may
+                  // start beside the pass; 0: the 256-row kernel does, which has no room there
 };
 constexpr int kWideRows = 256;
 // A share's slot: O as [rows][DP] in 32 bits, then (m, l) of each row.
@@ -124,18 +126,30 @@ __device__ __forceinline__ float weight(float m, float top) { return m == -INFIN
 // the latency of its start and end, and that one may start as soon as SMs are free (it is a
 // programmatic dependent).  A short prefix pass therefore yields: the SMs are shared out by the two
 // passes' work, measured by what an SM does of each in a nanosecond.  (32 sequences of 1-512 keys
-// behind 8192: 36 us, 53 without.  Over 8 units a block the passes slow each other more than the overlap
+// behind 8192: 36 us, 53 without; 8 tokens of each of 16 sequences of 1-500 keys behind 2000: 40, 56
+// without.  Over 8 units a block the passes slow each other more than the overlap
 // gives: 256 sequences behind 32768 keys 282 us against 267.)
 constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
 constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
 constexpr float kStartNs = 12000.f;                      // a launch of the pass, before and behind its units
 constexpr int kLeastKeys = 64;                           // that a sequence's own keys count for at least
 constexpr int kYieldUnits = 8;                           // of a block, up to which the prefix pass yields
-__device__ __forceinline__ bool yields(const PrefixShares& s, int line_units) { return line_units <= kYieldUnits * s.nc; }
+__device__ __forceinline__ bool brief(const PrefixShares& s, int line_units) { return line_units <= kYieldUnits * s.nc; }
+// Whether the prefix pass leaves SMs to the 16-row kernel; both go by this and by own_bytes.
+__device__ __forceinline__ bool yields(const PrefixShares& s, int line_units) { return s.own_shift > 0 && brief(s, line_units); }
 // What the pass takes on nc blocks a line.
 __device__ __forceinline__ float prefix_ns(const PrefixShares& s, int line_units, int nc) {
   return kStartNs + (float)((line_units + nc - 1) / nc) * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs);
 }
+// Items of a sequence in the 16-row kernel.
+constexpr int kRows = 16;  // query rows of one
+__device__ __forceinline__ int own_items(const Params& p) { return p.Hk * ((p.rows + kRows - 1) / kRows); }
+// Bytes of K and V that the 16-row kernel reads in `units` units, `items` of them a sequence at least.
+__device__ __forceinline__ float own_bytes(const Params& p, int units, int items) {
+  return fmaxf((float)units * (float)(1 << p.pre.own_shift), (float)p.B * items * kLeastKeys) * p.D * 4.f;
+}
+// Units of 2^shift keys (one at least, so that a sequence without keys gets its zeros).
+__device__ __forceinline__ int units_of(int keys, int shift) { return max(1, (keys + (1 << shift) - 1) >> shift); }
 // Blocks of a line that the prefix pass keeps beside `bytes` of the sequences' own keys.
 __device__ __forceinline__ int yielding_blocks(const PrefixShares& s, int sms, int line_units, float bytes) {
   const float mine = (float)line_units * s.lines * (s.tile == kWideRows ? kUnitNs : kHalfUnitNs), its = bytes / kSmBytesPerNs;

@@ -79,7 +79,6 @@ struct WideParams {
   int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
   int box_rows;    // rows of a page in one TMA box
   int lines;       // prefix pass: lines of units (paged_common.cuh)
-  int yields;      // prefix pass: may leave SMs to the kernel over the sequences' own keys
 };
 
 // An item's share of a block: blocks [j0, j1) of 128 keys of item (b, hk, pair).
@@ -374,20 +373,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     first.units = p.pre.units;
     const int items = p.Hk * (w.lines > 1 ? 1 : w.pairs), line_units = first.units * items;
     int nc = p.pre.nc;
-    const bool brief = yields(p.pre, line_units);
-    if (w.yields && brief) {
-      long long own = 0;
-      for (int b = threadIdx.x; b < p.B; b += kThreads) own += max(own_length(p, b), kLeastKeys);
+    if (yields(p.pre, line_units)) {
+      int* sums = reinterpret_cast<int*>(scratch);
+      int units = 0;  // of one item of each sequence
+      for (int b = threadIdx.x; b < p.B; b += kThreads) units += units_of(own_length(p, b), p.pre.own_shift);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(~0u, own, o);
-      if (lane == 0) scratch[warp] = own;
+      for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(~0u, units, o);
+      if (lane == 0) sums[warp] = units;
       __syncthreads();
-      own = 0;
+      units = 0;
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) own += scratch[i];
-      nc = yielding_blocks(p.pre, p.sms, line_units, (float)own * p.Hk * p.D * 4.f);
+      for (int i = 0; i < kThreads / 32; ++i) units += sums[i];
+      const int each = own_items(p);
+      nc = yielding_blocks(p.pre, p.sms, line_units, own_bytes(p, units * each, each));
     }
-    const int per_item = (brief || !w.yields) ? blocks_per_item(items, first.units, nc) : 0;
+    const int per_item = (brief(p.pre, line_units) || !p.pre.own_shift) ? blocks_per_item(items, first.units, nc) : 0;
     if (!per_item) {  // no more blocks than the longest share needs
       const int longest = up_div(line_units, nc);
       nc = up_div(line_units, longest);
@@ -1008,7 +1008,6 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   w.pairs = (int)((w.rows + tile - 1) / tile);
   w.box_rows = wide_box_rows(p.page_size);
   w.lines = 1;
-  w.yields = prefix_pass && p.rows <= 16;
   int64_t grid = sm_count();
   if (prefix_pass) {
     w.lines = p.pre.lines;

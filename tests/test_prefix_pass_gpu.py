@@ -137,3 +137,15 @@ def test_one_workspace_for_calls_of_all_forms():
         for c, (out, lse) in zip(cases, want):
             got = native(c, ws)
             assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 5, 8])
+def test_the_pass_yields_where_the_16_row_kernel_runs_beside_it(D, n):
+    """It leaves SMs to that kernel and to no other: up to 32 rows a sequence, where the block table is
+    narrow, and with a wide table (where the 256-row kernel takes the own keys) to none.  The own keys are
+    work enough for the pass to keep only half of its blocks."""
+    case = lambda: Case([1000] * 40, n=n, H=8, Hk=2, D=D, prefix=3000)  # noqa: E731
+    narrow, wide = native(case())[2], native(widen(case(), 512))[2]
+    assert narrow and wide
+    assert abs(narrow) < abs(wide) if n > 4 else narrow == wide
