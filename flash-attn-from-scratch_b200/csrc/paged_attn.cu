@@ -137,20 +137,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
   const int per_seq = own_items(p);
   const int c = blockIdx.x * kTeams + warp / kTeam;  // this warp's team
   Line line;
-  if (!locate<kThreads, kTeams>(
-          p.B, blockIdx.x * kTeams, reinterpret_cast<long long*>(sM), s_found, line,
-          [&](int b) { return (long long)units_of(p.prefix + own_length(p, b), kShift) * per_seq; },
-          [&](int units) {
-            // Beside a prefix pass that yields: as many blocks as run at once on the SMs it leaves (a
-            // second wave of them would begin when it ends), unless this pass is much the longer one.
-            const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
-            if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
-            const float bytes = own_bytes(p, units, per_seq);
-            const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
-            return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
-                                                                                           : (int)gridDim.x * kTeams;
-          }))
-    return;
+  locate<kThreads, kTeams>(
+      p.B, blockIdx.x * kTeams, reinterpret_cast<int*>(sM), s_found, line,
+      [&](int b) { return units_of(p.prefix + own_length(p, b), kShift) * per_seq; }, [&](int units) {
+        // Beside a prefix pass that yields: as many blocks as run at once on the SMs it leaves (a
+        // second wave of them would begin when it ends), unless this pass is much the longer one.
+        const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
+        if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
+        const float bytes = own_bytes(p, units, per_seq);
+        const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
+        return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
+                                                                                       : (int)gridDim.x * kTeams;
+      });
   if (c >= line.nc) return;
   Place<kShift> at;
   at.b = s_found[warp / kTeam].x;
@@ -480,6 +478,13 @@ int launch_join(const Params& p, cudaStream_t s) {
   return launch_kernel(paged_join_kernel<DP, kBf16>, (rows + kWarps - 1) / kWarps, kThreads, 0, true, s, p);
 }
 
+// Units of the line of a launch by teams of `team` warps, at most: sequences of at most `keys` keys.
+constexpr int64_t kMostUnits = 0x7FFFFFFF;
+int64_t line_units(int64_t items, int64_t keys, int team) {
+  const int64_t unit = 1 << team_shift(team);
+  return items * (keys > unit ? (keys + unit - 1) / unit : 1);
+}
+
 template <int DP, bool kBf16, int kTeam>
 int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
   using C = Cfg<DP>;
@@ -494,22 +499,24 @@ int launch_team(const Params& p, int64_t items, int64_t keys, cudaStream_t s) {
     configured.fetch_or(bit);
   }
   int64_t grid = 2 * (int64_t)sm_count();
-  constexpr int64_t kUnit = 1 << team_shift(kTeam), kTeams = kWarps / kTeam;
-  const int64_t most = items * (keys > kUnit ? (keys + kUnit - 1) / kUnit : 1);
+  constexpr int64_t kTeams = kWarps / kTeam;
+  const int64_t most = line_units(items, keys, kTeam);
   if (grid * kTeams > most) grid = (most + kTeams - 1) / kTeams;
   if (grid * kTeams > kPrefixBlocks) grid = kPrefixBlocks / kTeams;
   return launch_kernel(kern, (int)grid, kThreads, C::kSmem, p.row_share != nullptr, s, p);
 }
 
-// Warps of a team.
-int team_of(const Params& p) {
-  return (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows) >= kManyItems ? 1 : kWarps;
+// Warps of a team.  Lengths are device data: a line that might not fit 31 bits, by the block table's
+// width, takes the longer units of a team of four.
+int team_of(int64_t items, int64_t keys) {
+  return items >= kManyItems && line_units(items, keys, 1) <= kMostUnits ? 1 : kWarps;
 }
 
 template <int DP, bool kBf16>
 int launch_rows16(const Params& p, int64_t keys, cudaStream_t s) {
   const int64_t items = (int64_t)p.B * p.Hk * ((p.rows + kRows - 1) / kRows);
-  return team_of(p) == 1 ? launch_team<DP, kBf16, 1>(p, items, keys, s) : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
+  return team_of(items, keys) == 1 ? launch_team<DP, kBf16, 1>(p, items, keys, s)
+                                   : launch_team<DP, kBf16, kWarps>(p, items, keys, s);
 }
 
 }  // namespace paged
@@ -581,6 +588,22 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return LK_ERR_ALIGNMENT;
   for (int i = 0; i < 12; ++i)
     if (strides[i] % 8) return LK_ERR_ALIGNMENT;
+  // All lines of units fit 31 bits if that of the 16-row kernel by teams of four does: its units are no
+  // more keys or rows than any other's.  A batch for which it might not is taken in two halves.
+  const int64_t row_tiles = (n * (H / H_kv) + paged::kRows - 1) / paged::kRows;
+  if (paged::line_units(B * H_kv * row_tiles, prefix_length + table_cols * page_size, paged::kWarps) > paged::kMostUnits) {
+    if (B == 1) return LK_ERR_INVALID_ARG;
+    const int64_t half = B / 2;
+    for (int i = 0; i < 2; ++i) {
+      const int64_t b = i * half;
+      const int st = lk_shared_prefix_attention(
+          static_cast<const uint16_t*>(q) + b * strides[0], k_cache, v_cache, prefix_pages, prefix_length,
+          block_table ? block_table + b * table_ld : nullptr, table_ld, table_cols, lengths + b, static_cast<uint16_t*>(out) + b * strides[3], lse ? lse + b * n * H : nullptr, strides,
+          dtype, i ? B - half : half, n, H, H_kv, D, num_pages, page_size, softmax_scale, workspace, workspace_bytes, stream);
+      if (st != LK_OK) return st;
+    }
+    return LK_OK;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const DeviceScope scope(s);
   if (scope.status()) return scope.status();
@@ -608,7 +631,6 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   const int64_t DP = D > 64 ? 128 : 64;
   bool wide = paged::wide_box_rows(p.page_size) > 0;  // TMA can read the pages
   for (int i = 6; i < 12; ++i) wide = wide && strides[i] > 0;
-  const int64_t row_tiles = (p.rows + paged::kRows - 1) / paged::kRows;
   const bool pass = prefix_length > 0 && wide && B * row_tiles > 1 &&
                     B * H_kv * row_tiles * ((prefix_length + 63) / 64) > paged::kPrefixPass;
   const int64_t keys = (pass ? 0 : prefix_length) + table_cols * page_size;  // of a sequence, at most
@@ -616,9 +638,8 @@ extern "C" int lk_shared_prefix_attention(const void* q, const void* k_cache, co
   const bool own_wide = p.rows > paged::kRows && wide && (pass || prefix_length == 0) && !few;
   if (pass) {
     paged::PrefixShares pre = paged::prefix_shares(B * p.rows, H_kv, prefix_length);
-    if ((int64_t)pre.units * H_kv * pre.pairs > 0x7FFFFFFF) return LK_ERR_INVALID_ARG;
     pre.slots = p.partial + paged::own_floats(p.rows, DP);
-    pre.own_shift = own_wide ? 0 : paged::team_shift(paged::team_of(p));
+    pre.own_shift = own_wide ? 0 : paged::team_shift(paged::team_of(B * H_kv * row_tiles, keys));
     p.pre = pre;
     p.row_share = pre.slots + paged::prefix_floats(pre, H_kv, DP);
     if (int st = paged::launch_wide(p, bf16, true, 0, s)) return st;

@@ -173,34 +173,30 @@ struct Line {
 };
 
 // Finds where a block's teams (kTeams of them, consecutive on the line from team `team0`) begin, by
-// the whole block: units_of(b) is sequence b's count of units in 64 bits.  Two passes over the lengths: their
-// sum, by which the line is cut among most(sum) teams, and a scan up to the places looked for.  found[i] =
-// (sequence, unit among the sequence's) for team i.  Returns false (reported) if the line does not
-// fit 31 bits, which takes 2^37 keys.  scratch: 8-byte aligned, kThreads / 32 values.
+// the whole block: units_of(b) is sequence b's count of units; the host sees to it that the line fits
+// 31 bits.  Two passes over the lengths: their sum, by which the line is cut among most(sum) teams, and
+// a scan up to the places looked for.  found[i] = (sequence, unit among the sequence's) for team i.
+// scratch: kThreads / 32 values.
 template <int kThreads, int kTeams, class UnitsOf, class Most>
-__device__ __forceinline__ bool locate(int B, int team0, long long* scratch, int2* found, Line& line, UnitsOf units_of, Most most) {
+__device__ __forceinline__ void locate(int B, int team0, int* scratch, int2* found, Line& line, UnitsOf units_of, Most most) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long head = (int)threadIdx.x < B ? units_of((int)threadIdx.x) : 0;
-  long long mine = head;
+  const int head = (int)threadIdx.x < B ? units_of((int)threadIdx.x) : 0;
+  int mine = head;
   for (int b = threadIdx.x + kThreads; b < B; b += kThreads) mine += units_of(b);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
   if (lane == 0) scratch[warp] = mine;
   __syncthreads();
-  long long all = 0;
+  int all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) all += scratch[w];
-  if (all > 0x7FFFFFFF) {
-    record_bad_index(kSiteLength);
-    return false;
-  }
-  line.cut((int)all, max(1, most((int)all)));
+  line.cut(all, max(1, most(all)));
   const int last = line.begin(min(team0 + kTeams, line.nc) - 1);  // the last place looked for
   int base = 0;
   for (int b0 = 0; b0 < B && base <= last; b0 += kThreads) {
     const int b = b0 + (int)threadIdx.x;
-    const int n = (int)(b0 == 0 ? head : (b < B ? units_of(b) : 0));
+    const int n = b0 == 0 ? head : (b < B ? units_of(b) : 0);
     int scan = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -213,7 +209,7 @@ __device__ __forceinline__ bool locate(int B, int team0, long long* scratch, int
     int before = base, step = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const int x = (int)scratch[w];
+      const int x = scratch[w];
       if (w < warp) before += x;
       step += x;
     }
@@ -227,7 +223,6 @@ __device__ __forceinline__ bool locate(int B, int team0, long long* scratch, int
     base += step;
   }
   __syncthreads();
-  return true;
 }
 
 __device__ __forceinline__ int up_div(int a, int b) { return (int)((unsigned)(a + b - 1) / (unsigned)b); }

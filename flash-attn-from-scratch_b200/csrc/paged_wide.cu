@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = meet_bar + 1;    // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile Walk* walks = reinterpret_cast<volatile Walk*>(drain + 2);  // [8] of the softmax warps
-  long long* scratch = reinterpret_cast<long long*>(sQ);  // before the pipeline starts
+  int* scratch = reinterpret_cast<int*>(sQ);  // before the pipeline starts
 
   const int warp = warp_id();
   const int lane = threadIdx.x & 31;
@@ -374,16 +374,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int items = p.Hk * (w.lines > 1 ? 1 : w.pairs), line_units = first.units * items;
     int nc = p.pre.nc;
     if (yields(p.pre, line_units)) {
-      int* sums = reinterpret_cast<int*>(scratch);
       int units = 0;  // of one item of each sequence
       for (int b = threadIdx.x; b < p.B; b += kThreads) units += units_of(own_length(p, b), p.pre.own_shift);
 #pragma unroll
       for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(~0u, units, o);
-      if (lane == 0) sums[warp] = units;
+      if (lane == 0) scratch[warp] = units;
       __syncthreads();
       units = 0;
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) units += sums[i];
+      for (int i = 0; i < kThreads / 32; ++i) units += scratch[i];
       const int each = own_items(p);
       nc = yielding_blocks(p.pre, p.sms, line_units, own_bytes(p, units * each, each));
     }
@@ -428,10 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // after the other: units / nc + nc / items is least at this nc.  (64 tokens of 32/8
     // heads at 2000 keys: 43 us, against 53 where a join counts two units and 55 where it counts a half.)
     const float items = (float)p.B * p.Hk * w.pairs;
-    if (!locate<kThreads, 1>(
-            p.B, c, scratch, found, line, [&](int b) { return (long long)per_head(own_length(p, b)) * p.Hk; },
-            [&](int units) { return min((int)gridDim.x, (int)(sqrtf(units * items * (1.f / kJoinUnits)) + 1.f)); }))
-      return;
+    locate<kThreads, 1>(
+        p.B, c, scratch, found, line, [&](int b) { return per_head(own_length(p, b)) * p.Hk; },
+        [&](int units) { return min((int)gridDim.x, (int)(sqrtf(units * items * (1.f / kJoinUnits)) + 1.f)); });
     if (c >= line.nc) return;
     first.b = found->x;
     first.keys = own_length(p, first.b);

@@ -382,6 +382,9 @@ LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const v
  *              its first use; every call leaves its counters at zero again, so calls on one
  *              stream share it and calls that can overlap do not.  After a device failure (a
  *              wait that ran out) zero it again.
+ *   limits:    a sequence's tiles of 16 query rows times H_kv times the units of 64 keys that prefix_length
+ *              and table_cols * page_size allow for have to fit 31 bits (LK_ERR_INVALID_ARG); a batch
+ *              that passes them as a whole runs in parts.
  * Results do not depend on timing: the same call gives the same bits.
  *
  * lk_shared_prefix_attention: the same for a batch whose sequences share their first
