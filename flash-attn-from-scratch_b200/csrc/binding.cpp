@@ -355,7 +355,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       prefix = PyLong_AsLongLong(a[4]);
       if (prefix == -1 && PyErr_Occurred()) PyErr_Clear();
       require(prefix >= 0, "prefix_length must be an int >= 0");
-      require((prefix + kc.size(1) - 1) / kc.size(1) <= pages.size(0), "prefix_pages holds fewer than prefix_length keys");
+      require(prefix / kc.size(1) + (prefix % kc.size(1) != 0) <= pages.size(0), "prefix_pages holds fewer than prefix_length keys");
       same_device(pages, q);
       copy = copy || !(pages.stride(0) == 1 || pages.size(0) <= 1);
     }

@@ -149,3 +149,10 @@ def test_the_pass_yields_where_the_16_row_kernel_runs_beside_it(D, n):
     narrow, wide = native(case())[2], native(widen(case(), 512))[2]
     assert narrow and wide
     assert abs(narrow) < abs(wide) if n > 4 else narrow == wide
+
+
+@pytest.mark.parametrize("length", [33, 2 ** 31, 2 ** 63 - 1, 2 ** 63, 2 ** 70])
+def test_prefix_lengths_past_the_pages_are_refused(length):
+    c = Case([5, 9], prefix=32)
+    with pytest.raises(llm_kernels.LKInputError):
+        llm_kernels.shared_prefix_attention(c.q, c.k, c.v, c.prefix_pages, length, c.table, c.lengths)
