@@ -81,13 +81,30 @@ def _compile(src: str, verbose: bool) -> tuple[str, str]:
     return obj, (r.stderr if verbose else "")
 
 
+def _binding_includes() -> list[str] | None:
+    """Python's and torch's include folders, or None where the extension cannot be compiled: the C library
+    needs neither, nor g++."""
+    torch = importlib.util.find_spec("torch")
+    dirs = [sysconfig.get_paths()["include"]]
+    if torch is not None and torch.origin:
+        dirs.append(os.path.join(os.path.dirname(torch.origin), "include"))
+    wanted = ("Python.h", os.path.join("ATen", "dlpack.h"))
+    if shutil.which("g++") and all(any(os.path.exists(os.path.join(d, w)) for d in dirs) for w in wanted):
+        return dirs
+    return None
+
+
 def _build_binding(force: bool) -> None:
     src = os.path.join(CSRC, "binding.cpp")
     if not force and not _stale(BINDING, [src, OUT, *_headers()]):
         return
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    dirs = _binding_includes()
+    if dirs is None:
+        print("build.py: no g++, Python.h or torch (ATen/dlpack.h): llm_kernels/_binding.so, through which Python calls the "
+              "serving operators, is not built; the C library is", file=sys.stderr)
+        return
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
-           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(torch_dir, "include"), src, "-o", BINDING,
+           *("-I" + d for d in dirs), src, "-o", BINDING,
            "-L" + os.path.dirname(OUT), "-l:" + os.path.basename(OUT), "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

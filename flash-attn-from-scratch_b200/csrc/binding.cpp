@@ -443,13 +443,17 @@ PyObject* drop_workspaces(PyObject*, PyObject*) {
 // setup(torch.Tensor, empty_like, new_lse, capturing, zeros, LKInputError, call_error)
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count(n, 7)) return nullptr;
+  const char* no_api = "llm_kernels: this torch has no usable DLPack exchange functions";
   PyObject* capsule = PyObject_GetAttrString(a[0], "__dlpack_c_exchange_api__");
-  if (!capsule) return nullptr;
+  if (!capsule) {
+    PyErr_SetString(PyExc_ImportError, no_api);
+    return nullptr;
+  }
   const auto* api = static_cast<const DLPackExchangeAPI*>(PyCapsule_GetPointer(capsule, "dlpack_exchange_api"));
   Py_DECREF(capsule);  // the type holds it
   if (!api) return nullptr;
   if (api->header.version.major != DLPACK_MAJOR_VERSION || !api->dltensor_from_py_object_no_sync || !api->current_work_stream) {
-    PyErr_SetString(PyExc_ImportError, "llm_kernels: this torch has no usable DLPack exchange functions");
+    PyErr_SetString(PyExc_ImportError, no_api);
     return nullptr;
   }
   PyObject** to[] = {&g_tensor, &g_empty_like, &g_new_lse, &g_capturing, &g_zeros, &g_input_error, &g_call_error};

@@ -168,8 +168,15 @@ def binding():
         if _binding is None:
             import torch
 
-            from . import _binding as ext
             from ._common import LKInputError
+
+            try:
+                from . import _binding as ext
+            except ImportError as e:
+                raise ImportError(
+                    "llm_kernels: the extension of the serving operators (llm_kernels/_binding.so) is missing; build it with "
+                    "`python flash-attn-from-scratch_b200/build.py` where g++ and the headers of Python and torch are"
+                ) from e
 
             ext.setup(
                 torch.Tensor,
