@@ -250,11 +250,10 @@ int lk_version(void) { return (1 << 16) | 0; }
 
 int lk_set_device(int device) {
   using namespace lk;
-  if (device < 0 || device != t_device.device) {
-    int n = 0;
-    if (int st = cuda_status(cudaGetDeviceCount(&n))) return st;
-    if (device < 0 || device >= n) return cuda_status(cudaErrorInvalidDevice);
-  }
+  if (device >= 0 && device == t_device.device) return LK_OK;
+  int n = 0;
+  if (int st = cuda_status(cudaGetDeviceCount(&n))) return st;
+  if (device < 0 || device >= n) return cuda_status(cudaErrorInvalidDevice);
   t_device.device = device;
   t_device.seen = DeviceSwitch<CudaApi>::now();
   return LK_OK;

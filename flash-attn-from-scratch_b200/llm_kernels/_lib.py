@@ -215,7 +215,8 @@ def i64_array(vals) -> ctypes.Array:
 
 def set_device(index: int) -> None:
     """Picks the device of this thread's calls on the default stream; torch's current device stays."""
-    call("lk_set_device", int(index))
+    if (_lib or load()).lk_set_device(index) != LK_OK:  # on the way of every call
+        call("lk_set_device", index)
 
 
 def device_status() -> tuple[int, int, int, int]:

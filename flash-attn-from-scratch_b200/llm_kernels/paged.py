@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._common import require
-from .rotary import expand_positions, has_tangent
+from .rotary import dual_level, expand_positions, has_tangent
 
 __all__ = ["cache_slots", "paged_kv_append", "paged_attention", "shared_prefix_attention"]
 
@@ -60,10 +60,12 @@ def paged_kv_append(k, v, k_cache, v_cache, slots, *, q=None, positions=None, co
     Not differentiable: q, k or v that a derivative is asked of (grad mode with ``requires_grad``, or a
     forward-mode tangent) are refused.  Training rotates with :func:`rotary_embed`.
     """
-    grad = torch.is_grad_enabled()
-    for t in (k, v, q):
-        require(not (grad and getattr(t, "requires_grad", False)) and not has_tangent(t),
-                "paged_kv_append has no gradient: call it under torch.no_grad(), or rotate with rotary_embed to train")
+    try:
+        asked = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad))
+    except AttributeError:  # no tensor: refused below
+        asked = False
+    if asked or (dual_level() and (has_tangent(k) or has_tangent(v) or has_tangent(q))):
+        require(False, "paged_kv_append has no gradient: call it under torch.no_grad(), or rotate with rotary_embed to train")
     if sections is not None:
         sections = tuple(sections)
     append = _lib.binding().append

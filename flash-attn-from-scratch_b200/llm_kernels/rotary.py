@@ -82,9 +82,13 @@ class RotaryFunction(torch.autograd.Function):
         return rotate(tq, tk, positions, cos_sin, *ctx.how)
 
 
+def dual_level() -> bool:
+    """Whether a forward-mode level may be open (asked before a tensor is unpacked, which costs 0.35 us)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def has_tangent(x) -> bool:
-    # Without an open dual level there is none; that is asked first because unpacking costs 0.35 us.
-    return getattr(forward_ad, "_current_level", 0) >= 0 and isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None
+    return isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None
 
 
 def rotary_embed(q, k, positions, cos_sin, *, sections=None, interleaved=False, inverse=False):
@@ -110,11 +114,13 @@ def rotary_embed(q, k, positions, cos_sin, *, sections=None, interleaved=False, 
     require(isinstance(cos_sin, torch.Tensor) and not cos_sin.requires_grad, "cos_sin must be a tensor that needs no gradient")
     if sections is not None:
         sections = tuple(sections)
-    dual = has_tangent(q), has_tangent(k)
-    if k is not None and dual[0] != dual[1]:  # the function's outputs all have one, or none
-        return tuple(rotary_embed(x, None, positions, cos_sin, sections=sections, interleaved=interleaved, inverse=inverse)
-                     for x in (q, k))
-    if dual[0] or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+    dual = False
+    if dual_level():
+        dual = has_tangent(q)
+        if k is not None and dual != has_tangent(k):  # the function's outputs all have one, or none
+            return tuple(rotary_embed(x, None, positions, cos_sin, sections=sections, interleaved=interleaved, inverse=inverse)
+                         for x in (q, k))
+    if dual or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
         q_out, k_out = RotaryFunction.apply(q, k, positions, cos_sin, sections, interleaved, inverse)
     else:
         q_out, k_out = _rotate(q, k, positions, cos_sin, sections, interleaved, inverse)
