@@ -79,6 +79,9 @@ struct WideParams {
   int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
   int box_rows;    // rows of a page in one TMA box
   int lines;       // prefix pass: lines of units (paged_common.cuh)
+  // Test hook (lk_debug_inject): the barrier of block drop_block's ring item drop_item waits for more
+  // bytes than come.  drop_block = -1: none.
+  int drop_block, drop_item;
 };
 
 // An item's share of a block: blocks [j0, j1) of 128 keys of item (b, hk, pair).
@@ -502,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // a slot that is freed only when it is needed).
     bool ok = true;
     int issued = 0, fixes = 0;
+    const int drop = w.drop_block == (int)blockIdx.x ? w.drop_item : -1;
     const int box = w.box_rows, boxes = kBlockN / box;
     Item it = first;
     int j = j_first;
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mend = is_v && have < kBlockN && have > 0 && have % box != 0;
       uint64_t* bar = mend ? fix : &kv_full[slot];
       uint8_t* dst = sRing + slot * C::kTile;
-      if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+      if (lane == 0) mbar_arrive_expect_tx(bar, issued == drop ? C::kTile + 16 : C::kTile);
       __syncwarp();
       if (lane < boxes) {
         const CUtensorMap* tm = is_v ? &tmV : &tmK;
@@ -1006,6 +1010,11 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   w.pairs = (int)((w.rows + tile - 1) / tile);
   w.box_rows = wide_box_rows(p.page_size);
   w.lines = 1;
+  {
+    const Injection inj = take_injection(LK_INJECT_PAGED_DROP_LOAD);
+    w.drop_block = inj.kind ? inj.block : -1;
+    w.drop_item = inj.item;
+  }
   int64_t grid = sm_count();
   if (prefix_pass) {
     w.lines = p.pre.lines;

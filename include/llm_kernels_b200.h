@@ -93,14 +93,18 @@ LK_API int lk_debug_set_wait_limit(int64_t ns);
  *                                 `item`, warp slot 0, never publishes its partial;
  *   LK_INJECT_REQUANT_SKIP_PUBLISH  re-quantising GEMM: in CTA `block`, the epilogue warp of
  *                                 TMEM quadrant 0 never publishes its row maxima for its
- *                                 `item`-th tile, so that row block's codes warps wait in vain.
+ *                                 `item`-th tile, so that row block's codes warps wait in vain;
+ *   LK_INJECT_PAGED_DROP_LOAD     256-row paged attention (a prefix pass before the own keys): the
+ *                                 barrier of block `block`'s ring item `item` waits for more bytes
+ *                                 than come.
  * kind LK_INJECT_NONE disarms. */
 typedef enum {
   LK_INJECT_NONE = 0,
   LK_INJECT_FA_DROP_LOAD = 1,
   LK_INJECT_GEMM_DROP_LOAD = 2,
   LK_INJECT_SPLIT_SKIP_PUBLISH = 3,
-  LK_INJECT_REQUANT_SKIP_PUBLISH = 4
+  LK_INJECT_REQUANT_SKIP_PUBLISH = 4,
+  LK_INJECT_PAGED_DROP_LOAD = 5
 } lk_inject;
 LK_API int lk_debug_inject(int kind, int block, int item);
 
