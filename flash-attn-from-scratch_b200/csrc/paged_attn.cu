@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
         const int line_units = p.pre.units * (p.pre.lines > 1 ? p.Hk : p.Hk * p.pre.pairs);
         if (!p.row_share || !yields(p.pre, line_units)) return (int)gridDim.x * kTeams;
         const float bytes = own_bytes(p, units, per_seq);
-        const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / 8);
-        return bytes < 3.f * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
+        const int kept = yielding_blocks(p.pre, p.sms, line_units, bytes), left = max(p.sms - kept * p.pre.lines, p.sms / kLeastShare);
+        return bytes < kMuchLonger * left * kSmBytesPerNs * prefix_ns(p.pre, line_units, kept) ? left * 2 * kTeams
                                                                                        : (int)gridDim.x * kTeams;
       });
   if (c >= line.nc) return;
@@ -532,7 +532,10 @@ PrefixShares prefix_shares(int64_t rows, int64_t H_kv, int64_t prefix) {
   s.tile = rows <= kWideRows / 2 ? kWideRows / 2 : kWideRows;
   s.pairs = (int)((rows + s.tile - 1) / s.tile);
   s.units = (int)((prefix + 127) / 128);
-  // The pairs of a K/V head go side by side where that leaves at most a seventh of the SMs idle.
+  // The pairs of a K/V head go side by side where that leaves at most a seventh of the SMs idle: they read
+  // the same keys at the same time.  (32/8 heads, D = 128: 600 sequences behind 4096 keys, 10 pairs, 122 us
+  // against 127 on one line; 128 sequences of 100 own keys behind 4096, 2 pairs, 40 against 38.  With 30
+  // pairs, where 28 SMs would idle, 226 either way.)
   s.lines = s.pairs <= sms && sms / s.pairs * s.pairs * 7 >= sms * 6 ? s.pairs : 1;
   const int64_t items = s.lines > 1 ? H_kv : H_kv * s.pairs;
   s.nc = sms / s.lines;

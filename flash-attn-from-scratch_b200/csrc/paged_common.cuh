@@ -126,14 +126,38 @@ __device__ __forceinline__ float weight(float m, float top) { return m == -INFIN
 // the latency of its start and end, and that one may start as soon as SMs are free (it is a
 // programmatic dependent).  A short prefix pass therefore yields: the SMs are shared out by the two
 // passes' work, measured by what an SM does of each in a nanosecond.  (32 sequences of 1-512 keys
-// behind 8192: 36 us, 53 without; 8 tokens of each of 16 sequences of 1-500 keys behind 2000: 40, 56
-// without.  Over 8 units a block the passes slow each other more than the overlap
-// gives: 256 sequences behind 32768 keys 282 us against 267.)
-constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;  // an SM's time for a unit of 256 rows, of 128
-constexpr float kSmBytesPerNs = 60.f;                    // that an SM reads where memory is not shared by all
-constexpr float kStartNs = 12000.f;                      // a launch of the pass, before and behind its units
-constexpr int kLeastKeys = 64;                           // that a sequence's own keys count for at least
-constexpr int kYieldUnits = 8;                           // of a block, up to which the prefix pass yields
+// behind 8192: 34 us, 53 without; 8 tokens of each of 16 sequences of 1-500 keys behind 2000: 40, 56
+// without.)
+//
+// The constants' two sides, in us, as "sequences x tokens of own keys behind the prefix" (32/8 heads,
+// D = 128, single tokens where none are given; the constant's own value gives the figure in front).
+
+// An SM's time for a unit of 256 rows, of 128.  Also for D = 64, whose units hold half the work: with the
+// own keys counted twice beside them 64 x 5 of 1-500 behind 2000 (16/4 heads) 42, 50; 128 of 100 behind
+// 4096 27.6, 26.7.
+constexpr float kUnitNs = 2250.f, kHalfUnitNs = 1300.f;
+// Bytes that an SM reads in a nanosecond where memory is not shared by all.  At 30: 200 of 1-300 behind
+// 512 67, 77; 16 x 4 of 1-500 behind 4000 34, 30.  At 120: 16 x 8 of 1-500 behind 2000 40, 49; 32 of
+// 1-512 behind 8192 32, 36; 64 of 1-4096 behind 1024 135, 119.
+constexpr float kSmBytesPerNs = 60.f;
+// A launch of the pass, before and behind its units.  At 4000: 200 of 1-300 behind 512 67, 78.  At 36000:
+// 256 of 1-1024 behind 2048 160, 174; 64 of 1-4096 behind 1024 135, 119.
+constexpr float kStartNs = 12000.f;
+// Keys that a sequence's own count for at least.  At 16: 128 of 1-20 behind 3000 33, 36; 81 of 1-10 behind
+// 2000 30, 26.  At 256: 128 of 1-16 behind 8192 41, 58.
+constexpr int kLeastKeys = 64;
+// Units of a block up to which the prefix pass yields: longer ones slow the other pass more than the
+// overlap gives (256 of 16-1024 behind 32768 yielding 282, 263).  At 4: 128 of 1-16 behind 8192 41, 47;
+// 64 x 5 of 1-500 behind 2000 100, 92.  At 16, D = 64: 300 of 1-300 behind 8192 62, 65; 600 of 1-64
+// behind 4096 59, 52.
+constexpr int kYieldUnits = 8;
+// Times the prefix pass's that the own keys' may take on the SMs left to it; a longer one takes all SMs,
+// in the second wave of its blocks.  At 1: 32 of 1-2048 behind 8192 61, 66; 64 of 1-4096 behind 1024 at
+// D = 64 49, 68.  At 10: 256 of 1-1024 behind 2048 160, 173; 64 of 1-4096 behind 1024 135, 119.
+constexpr float kMuchLonger = 3.f;
+// The share of the SMs that the own keys' blocks are laid out for at least (they run behind the pass if
+// none are left).  At a third: 16 of none behind 16384 33, 37.  At 1/32, D = 64: the same 25, 29.
+constexpr int kLeastShare = 8;
 __device__ __forceinline__ bool brief(const PrefixShares& s, int line_units) { return line_units <= kYieldUnits * s.nc; }
 // Whether the prefix pass leaves SMs to the 16-row kernel; both go by this and by own_bytes.
 __device__ __forceinline__ bool yields(const PrefixShares& s, int line_units) { return s.own_shift > 0 && brief(s, line_units); }
@@ -232,7 +256,9 @@ __device__ __forceinline__ int up_div(int a, int b) { return (int)((unsigned)(a 
 // own (Q, the first S, and the way of O through memory), and in the even cut most blocks have the end of
 // one item and the begin of the next.  (32/8 heads: 16 sequences without own keys behind 16384 37 us against
 // 47, 128 of 1-20 keys behind 3000 33 against 49.  A long prefix pass beside single tokens keeps the even
-// cut, which leaves a few SMs more to them: 32 sequences behind 20000 keys 56 us against 58.)
+// cut, which leaves a few SMs more to them: 32 sequences behind 20000 keys 56 us against 58.  At 0 units
+// 32 sequences of 1-512 keys behind 8192 take 38 us against 32, and 256 of 1-1024 behind 2048 155 against
+// 160; at 3 nothing changes by 2%.)
 constexpr int kShareUnits = 1;
 __device__ __forceinline__ int blocks_per_item(int items, int units, int& nc) {
   if (items == 1 || items > nc) return 0;
