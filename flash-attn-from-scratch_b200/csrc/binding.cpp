@@ -77,6 +77,12 @@ void check(const char* name, int status) {
   throw Fail{};
 }
 
+bool flag(PyObject* o) {
+  const int yes = PyObject_IsTrue(o);
+  if (yes < 0) throw Fail{};
+  return yes != 0;
+}
+
 void* stream_on(const Tensor& t) {
   check("lk_set_device", lk_set_device(t.device.device_id));  // for the default stream, which names none
   void* s = nullptr;
@@ -196,6 +202,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       same_device(x[1], q);
     }
     const int64_t D = q.size(nd - 1);
+    const bool interleaved = flag(a[5]), inverse = flag(a[6]);
     Angles g;
     if (!angles(g, a[2], a[3], a[4], q.shape, nd - 2, D, q)) Py_RETURN_NONE;
     for (int i = 0; i < 2; ++i)
@@ -217,7 +224,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check("lk_rotary_embed",
           lk_rotary_embed(ptrs[0], ptrs[1], ptrs[2], ptrs[3], strides, q.code(), nd == 4 ? q.size(0) : 1, q.size(nd - 3),
                           heads[0], heads[1], D, g.positions, g.pos_type, g.pos_strides, g.table, g.rows, g.pairs, g.axes,
-                          g.sections, PyObject_IsTrue(a[5]), PyObject_IsTrue(a[6]), stream_on(q)));
+                          g.sections, interleaved, inverse, stream_on(q)));
     PyObject* r = PyTuple_New(2);
     if (!r) throw Fail{};
     PyTuple_SET_ITEM(r, 0, out[0].give());
@@ -276,6 +283,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 msg);
       }
     }
+    const bool interleaved = flag(a[9]);
     Angles g;
     if (a[7] != Py_None && !angles(g, a[6], a[7], a[8], k.shape, 1, D, k)) Py_RETURN_FALSE;
     if (!k.flat(2) || !v.flat(2) || !(slots.stride(0) == 1 || T <= 1) || (with_q && !q.flat(2))) Py_RETURN_FALSE;
@@ -291,7 +299,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
           lk_paged_kv_append(with_q ? q.ptr() : nullptr, with_q ? qo.ptr() : nullptr, k.ptr(), v.ptr(), kc.ptr(), vc.ptr(), st,
                              k.code(), T, with_q ? q.size(1) : 0, Hk, D, kc.size(0), kc.size(1), slots.ptr(), slots.code(),
                              g.positions, g.pos_type, g.pos_strides, g.table, g.rows, g.pairs, g.axes, g.sections,
-                             PyObject_IsTrue(a[9]), stream_on(k)));
+                             interleaved, stream_on(k)));
     return out.give();
   });
 }
@@ -380,7 +388,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       o = tensor(out.o, "");
       if (!strides_of(o, st + 3)) refuse("q must have rows on 16 bytes");
     }
-    const bool want_lse = PyObject_IsTrue(a[9]) == 1;
+    const bool want_lse = flag(a[9]);
     PyObject* none = Py_None;
     Ref lse(want_lse ? PyObject_CallOneArg(g_new_lse, a[0]) : Py_NewRef(none));
     if (B > 0 && n > 0 && H > 0) {
