@@ -24,10 +24,15 @@
 // the keys, joined at the item's end: the two tiles' warps see the same lanes of tensor memory).
 //
 // Measured (B200, 32/8 heads, D = 128, bf16): 2.2 us for a unit of 256 rows x 128 keys, as the
-// flash-attention forward takes (1100 TFLOP/s); 4 x 500 prompt tokens at up to 9000 keys 222 us (720
+// flash-attention forward takes (1100 TFLOP/s); 4 x 500 prompt tokens at up to 9000 keys 220 us (728
 // TFLOP/s: a share costs 15-20 thousand cycles besides its units, for Q, the first S, and the way of O
 // through memory where blocks share an item).  A launch of one unit takes 12 us, mostly instruction
 // fetches and round trips to memory that nothing hides yet.
+//
+// The softmax loop takes all 168 registers and spills a little: a warp makes 3 loads (5 where D = 64) and one
+// store of local memory a unit, measured by how those requests grow with the keys.  The probabilities are
+// rounded to the inputs' type for the second product, as in the flash-attention forward; kept in two parts
+// they would cost the tensor pipe half as much again.
 //
 // Keys behind a sequence's last one: whole boxes of them are not read (an out-of-range page
 // coordinate gives zeros); in the box that holds the end the rows of V behind it are zeroed in
@@ -79,9 +84,6 @@ struct WideParams {
   int halves;      // 2: tile 1 holds tile 0's queries and takes the odd key blocks
   int box_rows;    // rows of a page in one TMA box
   int lines;       // prefix pass: lines of units (paged_common.cuh)
-  // Test hook (lk_debug_inject): the barrier of block drop_block's ring item drop_item waits for more
-  // bytes than come.  drop_block = -1: none.
-  int drop_block, drop_item;
 };
 
 // An item's share of a block: blocks [j0, j1) of 128 keys of item (b, hk, pair).
@@ -505,7 +507,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // a slot that is freed only when it is needed).
     bool ok = true;
     int issued = 0, fixes = 0;
-    const int drop = w.drop_block == (int)blockIdx.x ? w.drop_item : -1;
     const int box = w.box_rows, boxes = kBlockN / box;
     Item it = first;
     int j = j_first;
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mend = is_v && have < kBlockN && have > 0 && have % box != 0;
       uint64_t* bar = mend ? fix : &kv_full[slot];
       uint8_t* dst = sRing + slot * C::kTile;
-      if (lane == 0) mbar_arrive_expect_tx(bar, issued == drop ? C::kTile + 16 : C::kTile);
+      if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
       __syncwarp();
       if (lane < boxes) {
         const CUtensorMap* tm = is_v ? &tmV : &tmK;
@@ -1010,11 +1011,6 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   w.pairs = (int)((w.rows + tile - 1) / tile);
   w.box_rows = wide_box_rows(p.page_size);
   w.lines = 1;
-  {
-    const Injection inj = take_injection(LK_INJECT_PAGED_DROP_LOAD);
-    w.drop_block = inj.kind ? inj.block : -1;
-    w.drop_item = inj.item;
-  }
   int64_t grid = sm_count();
   if (prefix_pass) {
     w.lines = p.pre.lines;
@@ -1022,9 +1018,12 @@ int launch_wide(const Params& p, bool bf16, bool prefix_pass, int64_t max_units,
   } else if (grid > max_units) {
     grid = max_units;
   }
+  // Test hook (lk_debug_inject): boxes of half the rows bring fewer bytes than the barriers wait for.
+  const Injection inj = take_injection(LK_INJECT_PAGED_DROP_LOAD);
+  auto rows_of = [&](int which) { return inj.kind && inj.item == which ? w.box_rows / 2 : w.box_rows; };
   CUtensorMap tk, tv;
-  if (int st = page_map(&tk, bf16, p.k, p, p.k_sp, p.k_ss, p.k_sh, w.box_rows)) return st;
-  if (int st = page_map(&tv, bf16, p.v, p, p.v_sp, p.v_ss, p.v_sh, w.box_rows)) return st;
+  if (int st = page_map(&tk, bf16, p.k, p, p.k_sp, p.k_ss, p.k_sh, rows_of(0))) return st;
+  if (int st = page_map(&tv, bf16, p.v, p, p.v_sp, p.v_ss, p.v_sh, rows_of(1))) return st;
   const bool dependent = !prefix_pass && p.row_share != nullptr;
   if (p.D > 64)
     return bf16 ? launch<128, true>(tk, tv, w, (int)grid, dependent, s) : launch<128, false>(tk, tv, w, (int)grid, dependent, s);

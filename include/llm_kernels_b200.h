@@ -94,9 +94,8 @@ LK_API int lk_debug_set_wait_limit(int64_t ns);
  *   LK_INJECT_REQUANT_SKIP_PUBLISH  re-quantising GEMM: in CTA `block`, the epilogue warp of
  *                                 TMEM quadrant 0 never publishes its row maxima for its
  *                                 `item`-th tile, so that row block's codes warps wait in vain;
- *   LK_INJECT_PAGED_DROP_LOAD     256-row paged attention (a prefix pass before the own keys): the
- *                                 barrier of block `block`'s ring item `item` waits for more bytes
- *                                 than come.
+ *   LK_INJECT_PAGED_DROP_LOAD     256-row paged attention (a prefix pass before the own keys): in every
+ *                                 block, half of each page of K (`item` 0) or V (1) is not loaded.
  * kind LK_INJECT_NONE disarms. */
 typedef enum {
   LK_INJECT_NONE = 0,
