@@ -19,9 +19,11 @@ import torch
 
 from . import _lib
 from ._common import require
-from .rotary import dual_level, expand_positions, has_tangent
+from .rotary import LEVEL, expand_positions, has_tangent
 
 __all__ = ["cache_slots", "paged_kv_append", "paged_attention", "shared_prefix_attention"]
+
+_grad_enabled = torch.is_grad_enabled
 
 def cache_slots(block_table: torch.Tensor, starts: torch.Tensor, new: int, page_size: int) -> torch.Tensor:
     """Slots of each sequence's next ``new`` tokens, ``[B * new]`` int64: sequence b's keys
@@ -61,10 +63,10 @@ def paged_kv_append(k, v, k_cache, v_cache, slots, *, q=None, positions=None, co
     forward-mode tangent) are refused.  Training rotates with :func:`rotary_embed`.
     """
     try:
-        asked = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad))
+        asked = _grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad))
     except AttributeError:  # no tensor: refused below
         asked = False
-    if asked or (dual_level() and (has_tangent(k) or has_tangent(v) or has_tangent(q))):
+    if asked or (LEVEL._current_level >= 0 and (has_tangent(k) or has_tangent(v) or has_tangent(q))):
         require(False, "paged_kv_append has no gradient: call it under torch.no_grad(), or rotate with rotary_embed to train")
     if sections is not None:
         sections = tuple(sections)

@@ -8,6 +8,8 @@ same kernel.
 
 from __future__ import annotations
 
+import types
+
 import torch
 from torch.autograd import forward_ad
 
@@ -82,9 +84,9 @@ class RotaryFunction(torch.autograd.Function):
         return rotate(tq, tk, positions, cos_sin, *ctx.how)
 
 
-def dual_level() -> bool:
-    """Whether a forward-mode level may be open (asked before a tensor is unpacked, which costs 0.35 us)."""
-    return getattr(forward_ad, "_current_level", 0) >= 0
+# The forward-mode level that is open, -1 without one (0, "ask the tensors", where torch keeps no such
+# number).  Asked first: to unpack a tensor costs 0.35 us.
+LEVEL = forward_ad if hasattr(forward_ad, "_current_level") else types.SimpleNamespace(_current_level=0)
 
 
 def has_tangent(x) -> bool:
@@ -115,7 +117,7 @@ def rotary_embed(q, k, positions, cos_sin, *, sections=None, interleaved=False, 
     if sections is not None:
         sections = tuple(sections)
     dual = False
-    if dual_level():
+    if LEVEL._current_level >= 0:
         dual = has_tangent(q)
         if k is not None and dual != has_tangent(k):  # the function's outputs all have one, or none
             return tuple(rotary_embed(x, None, positions, cos_sin, sections=sections, interleaved=interleaved, inverse=inverse)
