@@ -298,7 +298,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows16_kernel(const Params 
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = fa::ex2(fmaf(x[i >> 1][2 * h + (i & 1)], p.scale_log2, -ref));
         l[h] += (e[0] + e[1]) + (e[2] + e[3]);
-        // P is rounded to the inputs' type for the matrix product; the sum l is of the unrounded.
+        // P is rounded to the inputs' type for the matrix product; the sum l is of the unrounded.  (The
+        // error is then 1.35 times that of a result rounded once.  With P in two parts, and two products,
+        // 64 sequences of 200-8192 keys take 194 us instead of 188, one of 1000 keys 9.9 instead of 8.8.)
         pf[h] = pack2<kBf16>(e[0], e[1]);
         pf[2 + h] = pack2<kBf16>(e[2], e[3]);
       }

@@ -374,7 +374,9 @@ LK_API int lk_paged_kv_append(const void* q, void* q_out, const void* k, const v
  * h / (H / H_kv):
  *     out = softmax(scale q K^T) V,   lse[b][i][h] = ln sum_j exp(scale q.k_j)   (lse may be NULL)
  * A token that sees no key gives 0 and -inf.  Table entries past a sequence's last page are not
- * read; what lies behind its last key in a page never reaches the result.  A page id outside
+ * read; what lies behind its last key in a page never reaches the result.  (Among a call's newest
+ * tokens the mask is a zero probability, as in lk_flash_attn_fwd: a value that is not finite can reach
+ * the earlier ones of its sequence as 0 x Inf.)  A page id outside
  * [0, num_pages) counts as zeros and a length past table_cols * page_size is cut to that; both
  * are reported (lk_device_status).
  *   strides:   12 element strides: (b, n, h) of q and out, (page, row, h) of k_cache and v_cache,
