@@ -21,8 +21,8 @@
 // shared memory, a quarter as many go through the workspace), one where there are many (an item's
 // end then holds up one warp, not four).
 //
-// Measured (B200, 32/8 heads, D = 128, bf16): 64 sequences of 200-8192 keys 189 us, 5.9 TB/s of K
-// and V (a copy runs at 6.5); at 6000 keys each time grows by 6.6 TB/s, on top of 16-18 us that the
+// Measured (B200, 32/8 heads, D = 128, bf16): 64 sequences of 200-8192 keys 188-195 us, 5.8-5.9 TB/s of
+// K and V (a copy runs at 6.5); at 6000 keys each time grows by 6.6 TB/s, on top of 16-18 us that the
 // chain lengths -> table -> first keys, the joins and the launch take.  One sequence of 1000 keys:
 // 7.5 us, all of it such chains.
 #include <atomic>
@@ -43,18 +43,19 @@ constexpr float kLazy = 8.0f;  // log2 units that the maximum may grow by before
 // Units of 64 prefix keys, over all sequences, K/V heads and tiles of 16 query rows, above which the
 // prefix pass pays; below, each tile reads the prefix itself, mostly from L2, in one kernel.  One tile
 // alone shares nothing.  (32/8 heads, D = 128, one kernel against the pass.  16 single tokens: 256 keys
-// 15 us against 19, 1024 keys, 2048 units, 21 either way, 4096 keys 46 against 23.  20 tokens of each of
+// 17 us against 19, 1024 keys, 2048 units, 21 either way, 4096 keys 46 against 23.  20 tokens of each of
 // two sequences: 512 keys, 640 units, 19 either way, 4096 keys 38 against 25.  One piece of 500 tokens:
-// 64 keys 54 against 62, 256 keys, 4000 units, 64 either way, 8192 keys 487 against 124.  Of 252 calls
-// of 1-32 sequences, 1-500 tokens, 64-16384 keys and five head layouts the rule's choice takes 2.7% more
-// than the better one; at 2048 units it is 2.9%, at 6144 4.8%.)
+// 64 keys 53 against 61, 256 keys, 4000 units, 63 either way, 8192 keys 484 against 126.  Of 252 calls
+// of 1-32 sequences, 1-500 tokens, 64-16384 keys and five head layouts the rule's choice takes 2.5% more
+// than the better one, 41% at most; at 2048 units it is 2.7%, 96% at most, at 6144 4.5%.)
 constexpr int64_t kPrefixPass = 3072;
-// Items from which a team is one warp.  (64 sequences of 200-8192 keys, 8 K/V heads: 190 us against
-// 211 with teams of four; one sequence of 1000 keys: 20 against 7.5.)
+// Items from which a team is one warp.  (4 tokens of each of 16 sequences of 4-2999 keys, 16/16 heads, D = 64:
+// 31 us against 41 with teams of four; 32 sequences of 500 keys, 32/8 heads, 21 against 23; 64 of 6000 keys 266
+// against 270; one sequence of 1000 keys 23 with teams of one, 10 with teams of four.)
 constexpr int64_t kManyItems = 256;
 // Two tiles of 16 rows read their keys twice, but this kernel starts and joins faster than the one
 // of 256 rows: up to so many keys times K/V heads they take this one.  (32 rows: 8 heads of 8000 keys
-// 29 us against 52, 64 of 2000 35 against 43, 64 of 8000 102 against 78, 512 of 2000 189 against 154.)
+// 29 us against 54, 64 of 2000 33 against 44, 64 of 8000 104 against 83, 512 of 2000 191 against 156.)
 constexpr int64_t kTwoTileKeys = 1 << 18;
 
 template <int DP>

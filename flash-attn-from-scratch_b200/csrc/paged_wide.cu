@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // A share costs about a unit's time when it is joined, and the shares of an item are joined one
     // after the other: units / nc + nc / items is least at this nc.  (64 tokens of 32/8
-    // heads at 2000 keys: 43 us, against 53 where a join counts two units and 55 where it counts a half.)
+    // heads at 2000 keys: 44 us, against 54 where a join counts two units and 58 where it counts a half; at
+    // 8000 keys 81, 75 and 87.)
     const float items = (float)p.B * p.Hk * w.pairs;
     locate<kThreads, 1>(
         p.B, c, scratch, found, line, [&](int b) { return per_head(own_length(p, b)) * p.Hk; },
